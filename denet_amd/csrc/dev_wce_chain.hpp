@@ -32,10 +32,10 @@
 //     (sum_e e*g[e] = n*sum g - sum_e (g[0]+..+g[e])), so the inner loop is 3 packed instructions per
 //     2 (pixel, class) visits.
 //
-// Why packed: measured on MI355X (scripts/diag/valu_rate.hip), a SIMD issues one wave64 VALU instruction
-// per ~4.5 cycles whatever the wave count, v_pk_{mul,add,fma}_f32 cost the same slot as the plain forms and
-// v_exp_f32 costs two -- the kernel is bound by the instruction count, so two lanes of work per
-// instruction halve it.
+// The pairs: written on two-component vectors when v_pk_{mul,add,fma}_f32 still took the slot of one plain
+// instruction.  The build keeps the compiler from packed fp32 instructions (Makefile: some of their forms have given
+// wrong results); the plain ones measured, as whole steps at batch 8 / 20 / 8 of the three benchmark configurations,
+// 85.9 / 319.6 / 339.2 us against 86.4 / 321.1 / 331.1 us packed.
 //
 // Validity: every chain element is a true value exp2(y) with y in [min tap, 0]; a block whose shifted tap
 // logits all lie in [-120, 0] (log2 units: 83 nats below the tap's best class) can neither overflow nor lose

@@ -1,29 +1,24 @@
-// Diagnostic: VALU issue rate on gfx950 with 1..4 waves per SIMD: plain v_fma_f32 vs v_pk_fma_f32 vs v_exp_f32.
+// Diagnostic: VALU issue rate on gfx950 with 1..4 waves per SIMD: plain v_fma_f32 vs v_exp_f32.
 #include <hip/hip_runtime.h>
 #include <cstdio>
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 #define CK(x) do { hipError_t e = (x); if (e != hipSuccess) { printf("HIP error %s at %d\n", hipGetErrorString(e), __LINE__); return 1; } } while (0)
 template <int MODE>
 __global__ __launch_bounds__(256) void rate_kernel(float* out, int iters, float seed) {
     float a[8];
-    f32x2 p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { a[i] = seed + i + threadIdx.x; p[i] = {a[i], a[i] + 1.f}; }
+    for (int i = 0; i < 8; ++i) a[i] = seed + i + threadIdx.x;
     const float m = 1.0000001f;
-    const f32x2 m2 = {m, m};
     for (int it = 0; it < iters; ++it) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (MODE == 0) asm volatile("v_fma_f32 %0, %0, %1, %1" : "+v"(a[i]) : "v"(m));
-            if (MODE == 1) asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(p[i]) : "v"(m2));
             if (MODE == 2) asm volatile("v_exp_f32 %0, %0" : "+v"(a[i]));
-            if (MODE == 3) asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(p[i]) : "v"(m2));
             if (MODE == 4) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[i]) : "v"(m));
         }
     }
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += a[i] + p[i][0] + p[i][1];
+    for (int i = 0; i < 8; ++i) s += a[i];
     if (s == 12345.678f) out[0] = s;
 }
 template <int MODE>
@@ -51,8 +46,6 @@ int main() {
     float* out; CK(hipMalloc(&out, 4));
     run<0>("v_fma_f32", out);
     run<4>("v_mul_f32", out);
-    run<1>("v_pk_fma_f32", out);
-    run<3>("v_pk_mul_f32", out);
     run<2>("v_exp_f32", out);
     return 0;
 }
