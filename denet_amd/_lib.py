@@ -20,7 +20,7 @@ BWD_HAVE_FOCAL, BWD_NO_DFS, BWD_ONLY_DFS = 1, 2, 4      # denet_head_step_bwd fl
 # signature table: p = device pointer of any dtype (features, workspace; tensor / None),
 # F = device pointer to float32, L = device pointer to int64 (both checked against the tensor's dtype:
 # the kernels read raw memory, so a bf16 / half / int32 tensor would be misread without an error),
-# l = int64, u = uint64, i = int, f = float, h = host pointer (ctypes object / None)
+# l = int64, u = uint64, i = int, f = float, d = double, h = host pointer (ctypes object / None), a = host address (int)
 # the trailing stream argument is appended automatically ("s").
 _SIGS = {
     "denet_mask_resize": "L" "lllll" "FF",
@@ -51,6 +51,9 @@ _SIGS = {
     "denet_head_step_train_fwd": "ppi" "LLLLF" "FFFFFFF" "FF" "h" "lllllllll" "i" "FFF" "pl" "h",
     "denet_head_step_train_bwd": "piL" "FFF" "FF" "h" "F" "lllllllll" "pp" "FFFFFFF" "Fi" "pl" "h",
     "denet_dropout_mask": "uifl" "F",
+    "denet_grad_norm": "ald" "FF" "pl",
+    "denet_grad_clip": "ald" "F" "pl",
+    "denet_adamw_step": "alia" "F" "pl",
 }
 _NOSTREAM = {
     "denet_version": (ctypes.c_char_p, ""),
@@ -61,8 +64,10 @@ _NOSTREAM = {
     "denet_head_step_workspace": (ctypes.c_int64, "lllllllll"),
     "denet_upsample_loss_parts": (ctypes.c_int64, "llllli"),
     "denet_head_step_plan": (ctypes.c_int, "lllllllllih"),
+    "denet_opt_workspace": (ctypes.c_int64, "l"),
 }
-_CT = {"p": ctypes.c_void_p, "F": ctypes.c_void_p, "L": ctypes.c_void_p, "l": ctypes.c_int64, "u": ctypes.c_uint64, "i": ctypes.c_int, "f": ctypes.c_float, "h": ctypes.c_void_p}
+_CT = {"p": ctypes.c_void_p, "F": ctypes.c_void_p, "L": ctypes.c_void_p, "l": ctypes.c_int64, "u": ctypes.c_uint64, "i": ctypes.c_int, "f": ctypes.c_float, "h": ctypes.c_void_p,
+       "a": ctypes.c_void_p, "d": ctypes.c_double}
 
 
 class Probe(ctypes.Structure):
@@ -76,6 +81,17 @@ class Dropout(ctypes.Structure):
     reads the struct during each call, so a bound step sees a `seed` changed in place."""
     _fields_ = [("seed", ctypes.c_uint64), ("p_gate", ctypes.c_float), ("p_weight", ctypes.c_float)]
 
+
+class AdamWHyper(ctypes.Structure):
+    """denet_adamw_t (include/denet_hip.h)."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("max_norm", ctypes.c_double), ("device_steps", ctypes.c_int32),
+                ("reserved", ctypes.c_int32),
+                ("lr_dev", ctypes.c_void_p), ("coef", ctypes.c_void_p)]
+
+
+OPT_TENSOR_WORDS = 10       # denet_opt_tensor_t in 8-byte words
+OPT_QBLOCK = 256            # DENET_OPT_QBLOCK
 
 DROPOUT_GATE, DROPOUT_WEIGHT = 1, 2                     # stream ids of denet_dropout_mask
 
@@ -209,7 +225,7 @@ def _convert(name, args):
                 add(int(a))
         elif c == "h":
             add(None if a is None else ctypes.cast(ctypes.pointer(a), ctypes.c_void_p))
-        elif c == "f":
+        elif c in "fd":
             add(float(a))
         else:
             add(int(a))

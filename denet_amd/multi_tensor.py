@@ -1,0 +1,317 @@
+"""Operators over lists of tensors: the norm of a gradient list, its clipping, and the AdamW step (include/denet_hip.h, section O).
+
+A *plan* checks a list of tensors once and holds the table that the library reads at every call; like a bound step
+(`_lib.bind`) it keeps the tensors alive, and they stay in place (same storage, type and shape) while it is used.
+The functions without a plan check and pack the list at every call.
+
+Tensors are fp32 or bf16, dense (contiguous in some order of their dimensions, all tensors of one parameter in the same order),
+and of one device.  Calls go to torch's current stream of that device; norms are fresh 0-d fp32 tensors, workspaces come from
+torch's allocator at each call, so plans may be used on any stream and inside captured graphs.
+"""
+from __future__ import annotations
+
+import array
+import ctypes
+from bisect import bisect_right
+
+import torch
+
+from . import _lib
+from ._lib import DenetHipError
+
+_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_W = _lib.OPT_TENSOR_WORDS
+_STEP, _STEP_DEV = 7, 8                                  # word indices in denet_opt_tensor_t
+E4M3 = torch.float8_e4m3fn
+
+
+def _dense(t):
+    """Whether the elements fill one span of memory without gaps or overlaps, in some order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda x: x[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _check(t, what, types, device):
+    if not isinstance(t, torch.Tensor):
+        raise DenetHipError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.layout != torch.strided:
+        raise DenetHipError(f"{what}: sparse tensors are not supported")
+    if not t.is_cuda:
+        raise DenetHipError(f"{what}: denet_amd ops need device tensors (got a CPU tensor); there is no CPU path")
+    if t.dtype not in types:
+        raise DenetHipError(f"{what}: expected {' or '.join(str(x) for x in types)}, got {t.dtype}")
+    if t.device != device:
+        raise DenetHipError(f"{what}: on {t.device}, the list's first tensor is on {device}")
+    if not _dense(t):
+        raise DenetHipError(f"{what}: not dense (strides {tuple(t.stride())} of shape {tuple(t.shape)})")
+
+
+def _checked(tensors, what, types, device, index):
+    """The addresses of a list, every tensor checked (the first expression is `_check`'s fast form)."""
+    out = []
+    for i, t in enumerate(tensors):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in types and t.get_device() == index and
+                t.layout is torch.strided and t.is_contiguous()):
+            _check(t, f"{what} {i}", types, device)
+        out.append(t.data_ptr())
+    return out
+
+
+def _spans(tensors, addresses=None):
+    if addresses is None:
+        addresses = [t.data_ptr() for t in tensors]
+    return [(a, a + t.nbytes) for a, t in zip(addresses, tensors) if t.nbytes]
+
+
+def _check_overlap(written, read=()):
+    """Spans (first, last + 1): no byte may be written through two tensors, or written through one and read through another."""
+    written = sorted(written)
+    end = 0
+    for a, b in written:
+        if a < end:
+            raise DenetHipError("two tensors of the list overlap in memory (the same one twice, or views of the same elements)")
+        end = b
+    starts = [a for a, _ in written]
+    for a, b in read:
+        k = bisect_right(starts, b - 1) - 1
+        if k >= 0 and written[k][1] > a:
+            raise DenetHipError("a gradient shares memory with a tensor that the step writes")
+
+
+def _first_device(tensors, what):
+    if not tensors:
+        raise DenetHipError(f"{what}: an empty list of tensors")
+    t = tensors[0]
+    if not isinstance(t, torch.Tensor):
+        raise DenetHipError(f"{what}: expected a tensor, got {type(t).__name__}")
+    return t.device, t.get_device()
+
+
+class _Table:
+    """The host table of denet_opt_tensor_t rows and the calls on it."""
+
+    def __init__(self, rows, count, device, keep):
+        self.buf = array.array("q", rows)
+        self.addr = self.buf.buffer_info()[0]
+        self.count = count
+        self.device = device
+        self.index = device.index if device is not None else None
+        self.keep = keep
+        self.ws_bytes = _lib.query("denet_opt_workspace", count)
+
+    def ws(self):
+        return torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
+
+    def scalar(self):
+        return torch.empty((), dtype=torch.float32, device=self.device)
+
+    def call(self, name, *args):
+        """`args` end before the stream; raw addresses and numbers."""
+        fn = getattr(_lib.load(), name)
+        if self.index != torch.cuda.current_device():
+            with torch.cuda.device(self.index):
+                rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
+        else:
+            rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
+        if rc != 0:
+            raise DenetHipError(f"{name} failed: {_lib.strerror(rc)} (code {rc})")
+
+
+def _norm_limit(max_norm):
+    m = float(max_norm)
+    if not m >= 0.0:
+        raise DenetHipError(f"max_norm must be a number >= 0, got {max_norm}")
+    return m
+
+
+class GradNormPlan:
+    """The L2 norm over every element of a list of tensors, and clipping by it (torch.nn.utils.clip_grad_norm_)."""
+
+    def __init__(self, grads):
+        grads = list(grads)
+        device, index = _first_device(grads, "GradNormPlan")
+        addresses = _checked(grads, "gradient", _CODE, device, index)
+        rows = []
+        for g, a in zip(grads, addresses):
+            rows += (0, a, 0, 0, 0, 0, g.numel(), 1, 0, _CODE[g.dtype] << 32)
+        self.grads = grads
+        self._versioned = [g for g in grads if not g.is_inference()]
+        self._disjoint = False
+        self._table = _Table(rows, len(grads), device, grads)
+
+    def norm(self):
+        """sqrt(sum of squares), accumulated in 64 bits: a 0-d fp32 tensor."""
+        t = self._table
+        out, ws = t.scalar(), t.ws()
+        t.call("denet_grad_norm", -1.0, out.data_ptr(), None, ws.data_ptr(), t.ws_bytes)
+        return out
+
+    def norm_and_coef(self, max_norm):
+        """(norm, min(1, max_norm / (norm + 1e-6))) as 0-d fp32 tensors; the list is not written."""
+        limit = _norm_limit(max_norm)
+        t = self._table
+        out, coef, ws = t.scalar(), t.scalar(), t.ws()
+        t.call("denet_grad_norm", limit, out.data_ptr(), coef.data_ptr(), ws.data_ptr(), t.ws_bytes)
+        return out, coef
+
+    def clip_(self, max_norm):
+        """Scales the tensors in place by min(1, max_norm / (norm + 1e-6)); returns the norm before.  No tensor is touched where
+        the factor is 1."""
+        limit = _norm_limit(max_norm)
+        if not self._disjoint:
+            _check_overlap(_spans(self.grads))
+            self._disjoint = True
+        t = self._table
+        out, ws = t.scalar(), t.ws()
+        t.call("denet_grad_clip", limit, out.data_ptr(), ws.data_ptr(), t.ws_bytes)
+        if self._versioned:
+            torch.autograd.graph.increment_version(self._versioned)
+        return out
+
+
+class AdamWPlan:
+    """AdamW over a list of parameters.
+
+    exp_avgs / exp_avg_sqs: fp32 (m and v), or float8_e4m3fn codes of m and sqrt(v) with `exp_avg_scales` / `exp_avg_sq_scales`,
+    one fp32 scale per 256 consecutive elements of the parameter's memory (ceil(n / 256) each); zeros are the initial state.
+    steps: device int64 counters, one 0-d (or one-element) tensor per parameter, advanced by every `step()`; then `step` is not passed and
+    the call may be captured into a graph."""
+
+    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None, steps=None, _disjoint=False):
+        params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+        if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+            raise DenetHipError("AdamWPlan: scales for both states or for none")
+        self.bits = 32 if exp_avg_scales is None else 8
+        lists = [params, grads, exp_avgs, exp_avg_sqs]
+        if self.bits == 8:
+            lists += [list(exp_avg_scales), list(exp_avg_sq_scales)]
+        if steps is not None:
+            lists.append(list(steps))
+        n = len(params)
+        if any(len(x) != n for x in lists):
+            raise DenetHipError(f"AdamWPlan: lists of different lengths ({', '.join(str(len(x)) for x in lists)})")
+        device, index = _first_device(params, "AdamWPlan")
+        states = (torch.float32,) if self.bits == 32 else (E4M3,)
+        at = [_checked(x, what, types, device, index) for x, what, types in zip(
+            lists[:4], ("parameter", "gradient", "exp_avg", "exp_avg_sq"), (_CODE, _CODE, states, states))]
+        none = [0] * n
+        scales, counters = (none, none), none
+        sizes = [p.numel() for p in params]
+        for i, p in enumerate(params):
+            for t, what in ((grads[i], "gradient"), (exp_avgs[i], "exp_avg"), (exp_avg_sqs[i], "exp_avg_sq")):
+                if not (t.shape == p.shape and ((t.is_contiguous() and p.is_contiguous()) or t.stride() == p.stride())):
+                    raise DenetHipError(f"{what} {i}: shape {tuple(t.shape)} / strides {tuple(t.stride())}, the parameter has "
+                                        f"{tuple(p.shape)} / {tuple(p.stride())}")
+        if self.bits == 8:
+            scales = [_checked(x, what, (torch.float32,), device, index) for x, what in zip(lists[4:6], ("exp_avg scale", "exp_avg_sq scale"))]
+            for i, size in enumerate(sizes):
+                blocks = -(-size // _lib.OPT_QBLOCK)
+                for t, what in ((lists[4][i], "exp_avg scale"), (lists[5][i], "exp_avg_sq scale")):
+                    if t.numel() != blocks or not t.is_contiguous():
+                        raise DenetHipError(f"{what} {i}: {t.numel()} values, {blocks} are needed (one per {_lib.OPT_QBLOCK} elements)")
+                if size and (at[2][i] | at[3][i]) & 3:
+                    raise DenetHipError(f"8-bit states of parameter {i} do not start at a multiple of 4 bytes")
+        if steps is not None:
+            counters = _checked(lists[-1], "step counter", (torch.int64,), device, index)
+            if any(t.numel() != 1 for t in lists[-1]):
+                raise DenetHipError("step counters have one value each")
+        if not _disjoint:
+            written = [x for k in (0, 2, 3) for x in _spans(lists[k], at[k])]
+            written += [x for t in lists[4:] for x in _spans(t)]
+            _check_overlap(written, _spans(grads, at[1]))
+        codes = [_CODE[p.dtype] | (_CODE[g.dtype] << 32) for p, g in zip(params, grads)]
+        rows = [w for row in zip(at[0], at[1], at[2], at[3], scales[0], scales[1], sizes, [1] * n, counters, codes) for w in row]
+        self.device_steps = steps is not None
+        self._versioned = [t for t in params if not t.is_inference()]
+        self._table = _Table(rows, n, device, lists)
+        self._hyper = h = _lib.AdamWHyper()
+        h.device_steps = 1 if self.device_steps else 0
+        self._hyper_addr = ctypes.addressof(h)
+        self._lr = None
+        self._step = 1
+
+    def step(self, step=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, coef=None):
+        """One update.  step: the number t >= 1 of this update (an int, or one per parameter); not with device counters.  lr: a number, or (with
+        device counters) a one-element fp32 device tensor.  max_norm: clip by the norm of the gradients, which is
+        returned (the gradients themselves are not written).  coef: a one-element fp32 device tensor that multiplies the gradients instead."""
+        t, h = self._table, self._hyper
+        if self.device_steps:
+            if step is not None:
+                raise DenetHipError("AdamWPlan.step: this plan counts its steps on the device")
+        else:
+            if step is None:
+                raise DenetHipError("AdamWPlan.step: the number of the step is missing")
+            if torch.cuda.is_current_stream_capturing():
+                raise DenetHipError("AdamWPlan.step: a captured step would repeat its step number at every replay; give the plan "
+                                    "device step counters (`steps`)")
+            self._set_steps(step)
+        h.lr_dev = None
+        if isinstance(lr, torch.Tensor):
+            if not self.device_steps:
+                raise DenetHipError("AdamWPlan.step: lr as a tensor needs device step counters")
+            _check(lr, "lr", (torch.float32,), t.device)
+            if lr.numel() != 1:
+                raise DenetHipError(f"lr: {lr.numel()} values")
+            h.lr_dev = lr.data_ptr()
+            self._lr = lr
+        else:
+            h.lr = lr
+        h.beta1, h.beta2 = betas
+        h.eps, h.weight_decay = eps, weight_decay
+        h.coef = None
+        if coef is not None:
+            if max_norm is not None:
+                raise DenetHipError("AdamWPlan.step: max_norm or coef, not both")
+            _check(coef, "coef", (torch.float32,), t.device)
+            if coef.numel() != 1:
+                raise DenetHipError(f"coef: {coef.numel()} values")
+            h.coef = coef.data_ptr()
+        norm = ws = None
+        if max_norm is not None:
+            h.max_norm = _norm_limit(max_norm)
+            norm = t.scalar()
+        else:
+            h.max_norm = -1.0
+        if norm is not None or self.device_steps:
+            ws = t.ws()
+        t.call("denet_adamw_step", self.bits, self._hyper_addr, norm.data_ptr() if norm is not None else None,
+               ws.data_ptr() if ws is not None else None, t.ws_bytes if ws is not None else 0)
+        if self._versioned:
+            torch.autograd.graph.increment_version(self._versioned)
+        return norm
+
+    def _set_steps(self, step):
+        t = self._table
+        if isinstance(step, int):
+            if step != self._step:
+                if step < 1:
+                    raise DenetHipError(f"AdamWPlan.step: the first step is 1, got {step}")
+                t.buf[_STEP::_W] = array.array("q", [step]) * t.count
+                self._step = step
+            return
+        step = [int(s) for s in step]
+        if len(step) != t.count or min(step) < 1:
+            raise DenetHipError(f"AdamWPlan.step: {t.count} step numbers >= 1 are needed")
+        t.buf[_STEP::_W] = array.array("q", step)
+        self._step = None
+
+
+def grad_norm(grads):
+    """The L2 norm over every element of the tensors: a 0-d fp32 tensor."""
+    return GradNormPlan(grads).norm()
+
+
+def clip_grads_(grads, max_norm):
+    """Scales the tensors in place so that their common L2 norm is at most max_norm; returns the norm before."""
+    return GradNormPlan(grads).clip_(max_norm)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, exp_avg_scales=None, exp_avg_sq_scales=None, **hyper):
+    """AdamWPlan(...).step(step, **hyper) in one call."""
+    return AdamWPlan(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales).step(step, **hyper)

@@ -13,6 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import call, feat_code, query
+from .multi_tensor import AdamWPlan, GradNormPlan, adamw_step, clip_grads_, grad_norm      # noqa: F401  (the optimizer's operators)
 
 IGNORE_INDEX = 255
 DROPOUT_GATE, DROPOUT_WEIGHT = _lib.DROPOUT_GATE, _lib.DROPOUT_WEIGHT

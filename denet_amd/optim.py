@@ -1,0 +1,204 @@
+"""AdamW on the HIP kernels, with torch.optim's interface.
+
+Counterpart of the `torch.optim` classes that the reference's trainer builds by name (trainer/trainers.py:74-77) and steps
+(:973-975).  One launch updates up to 52 tensors; clipping by the global norm is folded into the step, which then reads the gradients a
+second time but never writes them.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import DenetHipError
+from .multi_tensor import E4M3, AdamWPlan, GradNormPlan, _check_overlap, _dense, _norm_limit, _spans
+
+__all__ = ["AdamW", "clip_grad_norm_"]
+
+
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ for the L2 norm: scales the `.grad`s in place, returns their norm before (0-d fp32 tensor).
+    error_if_nonfinite waits for the device, as there, and raises before anything is scaled."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    plan = GradNormPlan(grads)
+    _norm_limit(max_norm)
+    if error_if_nonfinite:
+        norm = plan.norm()
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the norm of the gradients is {float(norm)}, so they cannot be clipped")
+    return plan.clip_(max_norm)
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update (decoupled weight decay) on denet_adamw_step.
+
+    state_bits  32: exp_avg, exp_avg_sq in fp32 (also for bf16 parameters), interchangeable with torch.optim.AdamW's state.
+                 8: float8_e4m3fn codes exp_avg (of m) and exp_avg_sqrt (of sqrt(v)) in the parameter's shape, with
+                    exp_avg_scale / exp_avg_sqrt_scale, one fp32 scale per 256 consecutive elements of its memory.
+    max_norm    clip by the norm of all gradients of all groups, as clip_grad_norm_ before the step would; `grad_norm` then holds the norm.
+    capturable  steps are counted on the device (state 'step': 0-d int64), so that step() may be captured into a graph and replayed; lr may
+                then be a one-element fp32 tensor on the device.  Capture after one eager step, which creates the state.
+
+    Parameters are fp32 or bf16 on one GPU, dense in some order of their dimensions; gradients in another order or type are converted."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.state_bits, self.capturable = state_bits, bool(capturable)
+        self.max_norm = None if max_norm is None else _norm_limit(max_norm)       # may be changed between steps
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    # ---- checks ------------------------------------------------------------------------------
+    def _check_group(self, group):
+        lr, betas = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor):
+            if not self.capturable:
+                raise ValueError("lr as a tensor needs capturable=True")
+        elif not float(lr) >= 0.0:
+            raise ValueError(f"invalid learning rate: {lr}")
+        if len(betas) != 2 or not all(0.0 <= float(b) < 1.0 for b in betas):
+            raise ValueError(f"invalid betas: {betas}")
+        if not float(group["eps"]) >= 0.0 or not float(group["weight_decay"]) >= 0.0:
+            raise ValueError(f"invalid eps / weight_decay: {group['eps']}, {group['weight_decay']}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            self._check_group(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise ValueError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+                if p.layout != torch.strided or not _dense(p):
+                    raise ValueError("parameters must be dense in memory")
+            _check_overlap(_spans([p for g in self.param_groups for p in g["params"]]))
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    # ---- state ---------------------------------------------------------------------------------
+    def _state_of(self, p):
+        s = self.state[p]
+        if not s:
+            if self.state_bits == 8:
+                blocks = -(-p.numel() // _lib.OPT_QBLOCK)
+                for key in ("exp_avg", "exp_avg_sqrt"):
+                    s[key] = torch.empty_like(p, dtype=E4M3).view(torch.uint8).zero_().view(E4M3)
+                    s[key + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+            else:
+                for key in ("exp_avg", "exp_avg_sq"):
+                    s[key] = torch.zeros_like(p, dtype=torch.float32)
+            s["step"] = torch.zeros((), dtype=torch.int64, device=p.device) if self.capturable else 0
+        return s
+
+    @staticmethod
+    def _grad_of(p):
+        g = p.grad
+        if g.is_sparse or g.layout != torch.strided:
+            raise DenetHipError("AdamW: sparse gradients are not supported")
+        if g.dtype not in (torch.float32, torch.bfloat16):
+            g = g.float()
+        if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        return g
+
+    # ---- the step --------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise DenetHipError("AdamW: a captured step() needs capturable=True (its step numbers would be repeated by every replay)")
+        eight = self.state_bits == 8
+        work = []
+        for group in self.param_groups:
+            self._check_group(group)
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            if capturing and any(not self.state[p] for p in params):
+                raise DenetHipError("AdamW: run one eager step before the capture (it creates the state)")
+            work.append((group, params, [self._grad_of(p) for p in params], [self._state_of(p) for p in params]))
+        if not work:
+            self.grad_norm = None
+            return loss
+        plans = []
+        for group, params, grads, states in work:
+            keys = ("exp_avg", "exp_avg_sqrt", "exp_avg_scale", "exp_avg_sqrt_scale") if eight else ("exp_avg", "exp_avg_sq")
+            plans.append(AdamWPlan(params, grads, *([s[k] for s in states] for k in keys),
+                                   steps=[s["step"] for s in states] if self.capturable else None, _disjoint=True))
+        max_norm, coef = self.max_norm, None
+        self.grad_norm = None
+        if max_norm is not None and len(work) > 1:
+            # one norm over all groups: its coefficient is left on the device for the groups' calls
+            self.grad_norm, coef = GradNormPlan([g for w in work for g in w[2]]).norm_and_coef(max_norm)
+            max_norm = None
+        for (group, params, _, states), plan in zip(work, plans):
+            step = None
+            if not self.capturable:
+                for s in states:
+                    s["step"] += 1
+                step = [s["step"] for s in states]
+                if min(step) == max(step):
+                    step = step[0]
+            norm = plan.step(step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                             max_norm=max_norm, coef=coef)
+            if max_norm is not None:
+                self.grad_norm = norm
+        return loss
+
+    # ---- checkpoints --------------------------------------------------------------------------------
+    def load_state_dict(self, state_dict):
+        """Takes its own state_dict and, with 32-bit states, torch.optim.AdamW's.  States keep their types (the base class would cast
+        them to the parameter's)."""
+        saved_groups, saved = state_dict["param_groups"], state_dict["state"]
+        if len(saved_groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"])
+                                                              for a, b in zip(saved_groups, self.param_groups)):
+            raise ValueError("the saved state has other parameter groups than this optimizer")
+        for g in saved_groups:
+            if not all(k in g for k in self.defaults) or g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("the saved parameter groups are not those of an AdamW without amsgrad / maximize")
+        by_id = dict(zip((i for g in saved_groups for i in g["params"]), (p for g in self.param_groups for p in g["params"])))
+        fresh = {p: self._converted(p, saved[i]) for i, p in by_id.items() if i in saved and saved[i]}
+        super().load_state_dict({"state": {}, "param_groups": [{k: v for k, v in g.items() if k in ("params", "initial_lr") or k in self.defaults}
+                                                               for g in saved_groups]})
+        for p, s in fresh.items():
+            self.state[p] = s
+
+    def _converted(self, p, s):
+        if self.state_bits == 8:
+            types = {"exp_avg": E4M3, "exp_avg_sqrt": E4M3, "exp_avg_scale": torch.float32, "exp_avg_sqrt_scale": torch.float32}
+        else:
+            types = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32}
+        if not all(k in s for k in (*types, "step")) or (self.state_bits == 32 and "exp_avg_scale" in s):
+            raise ValueError(f"the saved state ({', '.join(sorted(s))}) is not that of an AdamW with {self.state_bits}-bit states")
+        out = {}
+        for k, dtype in types.items():
+            v = s[k].detach().to(p.device)
+            if k.endswith("_scale"):
+                if v.shape != (-(-p.numel() // _lib.OPT_QBLOCK),) or v.dtype != dtype:
+                    raise ValueError(f"{k}: {tuple(v.shape)} {v.dtype} does not belong to a parameter of {p.numel()} elements")
+                out[k] = v.contiguous().clone()
+            elif v.shape != p.shape:
+                raise ValueError(f"{k}: shape {tuple(v.shape)}, the parameter has {tuple(p.shape)}")
+            elif self.state_bits == 8:
+                # codes belong to blocks of consecutive MEMORY: another order of the dimensions would regroup them
+                if v.dtype != E4M3 or not (v.stride() == p.stride() or (v.is_contiguous() and p.is_contiguous())):
+                    raise ValueError(f"{k}: saved as {v.dtype} with strides {tuple(v.stride())}, the parameter has {tuple(p.stride())}")
+                out[k] = v.clone()
+            else:
+                out[k] = torch.empty_like(p, dtype=dtype).copy_(v)
+        step = int(s["step"])
+        out["step"] = torch.full((), step, dtype=torch.int64, device=p.device) if self.capturable else step
+        return out
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for k, v in (("state_bits", 32), ("capturable", False), ("max_norm", None), ("grad_norm", None)):
+            self.__dict__.setdefault(k, v)

@@ -46,6 +46,7 @@ from . import ops, sharding
 from .head import DENet, freeze_weights, get_architecture, key2arch
 from .losses import get_loss, loss_denet_batch
 from .metrics import BinaryIOU as bIOU, FullIOU as fIOU
+from .optim import AdamW as FusedAdamW
 from .schedulers import get_scheduler, tick
 from .synthetic import EpisodeShape, make_episodes
 
@@ -196,8 +197,10 @@ def nway_fusion_update(b_iou, pre, Yq, cls_idx, way, order_base=None):
 
 
 def _make_optimizer(name, params, **cfg):
+    """The reference's names (trainer/trainers.py:74-77) are torch's own classes; `fused_adamw` (an extension; options
+    `state_bits: 8 | 32`) is this package's AdamW on the HIP kernels."""
     table = {'sgd': torch.optim.SGD, 'adam': torch.optim.Adam, 'adamw': torch.optim.AdamW,
-             'rmsprop': torch.optim.RMSprop, 'adagrad': torch.optim.Adagrad}
+             'rmsprop': torch.optim.RMSprop, 'adagrad': torch.optim.Adagrad, 'fused_adamw': FusedAdamW}
     if name.lower() not in table:
         raise NotImplementedError('Optimizer {} not implemented'.format(name))
     return table[name.lower()](params, **cfg)
@@ -239,6 +242,15 @@ class DENetTrainer(object):
                                              **opt)
             self.scheduler = get_scheduler(self.optimizer, scheduler_dict=self.train_cfg.get('scheduler', None))
             self.bucket = sharding.GradBucket(self.model.parameters())
+            # train.max_grad_norm (an extension): clip by the norm of all (rank-averaged) gradients; fused_adamw takes the
+            # factor into its own pass, any other optimizer gets the flat bucket scaled before it steps
+            self.grad_norm, self._clip = None, None
+            self.max_grad_norm = self.train_cfg.get('max_grad_norm')
+            if self.max_grad_norm is not None:
+                if isinstance(self.optimizer, FusedAdamW):
+                    self.optimizer.max_norm = float(self.max_grad_norm)
+                else:
+                    self._clip = ops.GradNormPlan([self.bucket.flat])
             self.loss_func = DENet_loss_wrapper(get_loss(self.train_cfg['loss']), arch=arch)
             self.num_steps = self.train_cfg['num_steps']
             self.log_steps = self.train_cfg.get('log_steps', 10)
@@ -329,7 +341,11 @@ class DENetTrainer(object):
             self.bucket.zero()
             loss_k.backward()                       # only the knowledge loss (trainer/trainers.py:972-974)
             self.bucket.all_reduce_mean()
+            if self._clip is not None:
+                self.grad_norm = self._clip.clip_(self.max_grad_norm)
             self.optimizer.step()
+            if isinstance(self.optimizer, FusedAdamW):
+                self.grad_norm = self.optimizer.grad_norm
         lk, lp = torch.stack([loss_k.detach(), loss_p.detach()]).tolist()     # one host sync
         return out_b.detach(), out_f.detach(), lk + lp, lk, lp
 

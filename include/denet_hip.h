@@ -370,6 +370,65 @@ int denet_head_step_train_bwd(const void* Fq, int feat_dtype, const int64_t* lab
                         float* db2, float* dWl, float* dbl, float* losses, int flags,
                         void* ws, int64_t ws_bytes, const denet_probe_t* probe, void* stream);
 
+/* ---- O: the optimizer step over many tensors ------------------------------------
+ * What DENetTrainer does between loss_k.backward() and the next step: clip_grad_norm_ and AdamW over the
+ * parameter list (the reference takes its optimizers from torch.optim: trainer/trainers.py:74-77,973-975).
+ *   norm  = sqrt(sum over all tensors and elements of g^2), accumulated in 64 bits
+ *   coef  = min(1, max_norm / (norm + 1e-6))     (a NaN norm gives a NaN coefficient, an infinite one 0)
+ *   g'    = coef * g
+ *   m    <- beta1 m + (1 - beta1) g';   v <- beta2 v + (1 - beta2) g'^2
+ *   p    <- (1 - lr weight_decay) p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32, each operation rounded by itself; bf16 parameters and gradients are widened on load, and bf16 parameters
+ * rounded to nearest even once.
+ *
+ * `tensors` is a HOST array, read during the call (it travels as kernel arguments: nothing is copied to the device, a
+ * captured graph holds its own copy).  Tensors with n = 0 are skipped.  param, grad, the 32-bit states and the scales need the alignment of
+ * their element, 8-bit codes that of 4 bytes.  No two written ranges may overlap.
+ *
+ * bits = 32: exp_avg = m, exp_avg_sq = v, float [n]; avg_scale / sq_scale unused.
+ * bits = 8:  exp_avg / exp_avg_sq hold one e4m3 code per element, of m / s and of sqrt(v) / s, with one float s for each
+ *            256 consecutive elements of the tensor (the last block may be shorter): avg_scale / sq_scale [ceil(n / 256)],
+ *            s = max(largest finite magnitude of the block * (1.f / 448), 2^-126).  sqrt(v) > 0 takes at least the
+ *            smallest code.  An entry that is not finite takes the NaN code.  The update of p uses the moments before
+ *            they are rounded.  All-zero codes and scales are the initial state.
+ *
+ * ws: denet_opt_workspace(count) bytes, 8-byte aligned, written by every call that takes a norm or device-side
+ * steps (calls that overlap in time need one each); adamw_step without either may pass NULL. */
+#define DENET_OPT_QBLOCK 256
+typedef struct denet_opt_tensor {
+    void* param;            /* DENET_F32 / DENET_BF16 [n] (unused by grad_norm / grad_clip)      */
+    void* grad;             /* DENET_F32 / DENET_BF16 [n]; written by grad_clip only              */
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* avg_scale;
+    float* sq_scale;
+    int64_t n;              /* elements, < 2^48                                                   */
+    int64_t step;           /* t >= 1 of this update                                              */
+    int64_t* step_dev;      /* with denet_adamw_t.device_steps: device counter of the updates done so far, advanced by
+                               the call, in place of `step` -- for calls that a captured graph replays */
+    int32_t param_dtype;
+    int32_t grad_dtype;
+} denet_opt_tensor_t;
+typedef struct denet_adamw {
+    double lr, beta1, beta2, eps, weight_decay;
+    double max_norm;        /* < 0: no clipping; else the norm of the list is taken first and g' = coef g (grads themselves
+                               are not written)                                                   */
+    int32_t device_steps;   /* 1: the tensors' step_dev count                                      */
+    int32_t reserved;
+    const float* lr_dev;    /* with device_steps: device scalar read instead of lr, or NULL        */
+    const float* coef;      /* device scalar: coefficient that denet_grad_norm left, where one norm spans several
+                               calls (parameter groups); or NULL.  Not together with max_norm >= 0 */
+} denet_adamw_t;
+int64_t denet_opt_workspace(int64_t count);
+/* norm; and coef for max_norm where asked for */
+int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm /*[1]*/,
+                    float* coef /*[1] or NULL*/, void* ws, int64_t ws_bytes, void* stream);
+/* norm, and g <- coef * g in place */
+int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm /*[1]*/, void* ws,
+                    int64_t ws_bytes, void* stream);
+int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, int bits, const denet_adamw_t* h /* HOST */,
+                     float* norm /*[1], with clipping; else NULL*/, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

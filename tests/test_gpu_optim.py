@@ -1,0 +1,769 @@
+"""GPU: the operators over lists of tensors (gradient norm, clipping, AdamW with 32- and 8-bit states) against their formulas in 64 bits,
+against the same fp32 arithmetic written with elementary tensor operations (bit for bit), and driven together through the optimizer and
+the trainer.
+
+Tolerances: u = 2^-24 is half a step of fp32.  Counting the roundings of each formula (constants are rounded once too):
+  coef         fp64 throughout, rounded once                               u
+  g' = coef g                                                              2 u |g'|
+  m' = m b1 + g' c1      products 2 u each (+ 2 u of g'), sum u            5 u (|m b1| + |g' c1|)        =: em
+  v' = v b2 + g'^2 c2    2 u; 2*2 + 1 + 2 u; sum u                         8 u (v b2 + g'^2 c2)
+  r' = sqrt(v')          half of it + u                                    5 u r'
+  d  = r' k + eps        5 + 2, eps u, sum u                               8 u d
+  p' = p D - (m'/d) S    p: 2 u; quotient em/d + (8 + 1) u, times S 2 u; sum u
+with 8-bit states m, r are code * scale (one more u each; r twice in v): 6 and 10 in place of 5 and 8."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+TINY = 2.0 ** -126
+SIZES = [1, 3, 255, 256, 257, 1024, 4095, 4096, 4097, 13001, 70003]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    return torch.device("cuda:0")
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+# ---- norm and clipping ---------------------------------------------------------------------------------
+def _grads(sizes, types, dev, seed, offset=0):
+    """Views into one slab per type, packed from element `offset` on, with a guard behind them."""
+    g = _gen(dev, seed)
+    slabs = {t: torch.full((offset + sum(sizes) + 64,), 7.0, dtype=t, device=dev) for t in set(types)}
+    at, out = dict.fromkeys(slabs, offset), []
+    for i, n in enumerate(sizes):
+        t = types[i % len(types)]
+        v = slabs[t][at[t]:at[t] + n]
+        v.copy_(torch.randn(n, device=dev, generator=g) * 10.0 ** (i % 5 - 3))
+        at[t] += n
+        out.append(v)
+    return out, slabs, at
+
+
+def _norm64(ts):
+    return math.sqrt(sum(float(t.double().square().sum()) for t in ts))
+
+
+@pytest.mark.parametrize("sizes,types,offset", [
+    ([1], [F32], 0), ([1], [BF16], 1), ([0, 5], [F32], 1), (SIZES, [F32], 0), (SIZES, [F32], 3), (SIZES, [BF16], 1),
+    (SIZES, [F32, BF16], 5), ([7] * 64, [F32], 0), ([9] * 65, [BF16, F32], 1), ([11, 5000] * 150, [F32, BF16], 1), ([5_000_011], [F32], 1),
+    ([4096 * 1030], [BF16], 0), ([2_000_003, 3_000_017] * 2, [BF16, F32], 1)])
+def test_norm(sizes, types, offset, dev):
+    from denet_amd import ops
+    grads, _, _ = _grads(sizes, types, dev, 1, offset)
+    plan = ops.GradNormPlan(grads)
+    n = plan.norm()
+    want = _norm64(grads)
+    assert n.dtype == F32 and n.shape == ()
+    assert abs(float(n) - want) <= 1.01 * U * want
+    assert torch.equal(plan.norm(), n)                                        # same order of sums at every call
+    n2, coef = plan.norm_and_coef(0.37 * want)
+    assert torch.equal(n2, n) and abs(float(coef) - 0.37) <= (0.37 * 2 * U + 1e-6 / want)
+    assert float(plan.norm_and_coef(2.0 * want + 1)[1]) == 1.0
+
+
+def test_norm_extremes(dev):
+    from denet_amd import ops
+    for v in (1e30, 3e38, 1e-30, 2.0 ** -149):
+        x = torch.full((1000,), v, device=dev)
+        want = _norm64([x])
+        # 1000 * 3e38^2 is far beyond fp32; a result beyond fp32's largest number is infinite
+        got = float(ops.grad_norm([x]))
+        assert got == math.inf if want > 3.4028235e38 else abs(got - want) <= 2 * U * want + 2.0 ** -149
+    x = torch.ones(5000, device=dev)
+    x[4321] = math.inf
+    assert float(ops.grad_norm([torch.ones(3, device=dev), x])) == math.inf
+    x[17] = math.nan
+    assert math.isnan(float(ops.grad_norm([x])))
+    z = torch.zeros(0, device=dev)
+    assert float(ops.grad_norm([z])) == 0.0 and float(ops.clip_grads_([z, z], 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("types", [[F32], [BF16], [BF16, F32]])
+@pytest.mark.parametrize("share", [0.0, 0.25, 0.999, 1.0, 3.0])
+def test_clip(types, share, dev):
+    from denet_amd import ops
+    grads, slabs, at = _grads(SIZES * 7, types, dev, 2, 1)
+    before = [g.clone() for g in grads]
+    want = _norm64(grads)
+    limit = share * want + (1e-3 if share >= 1 else 0.0)
+    versions = [g._version for g in grads]
+    norm = ops.clip_grads_(grads, limit)
+    assert abs(float(norm) - want) <= 1.01 * U * want
+    c = min(1.0, limit / (want + 1e-6))
+    half = 2.0 ** -8
+    for g, b in zip(grads, before):
+        ref = b.double() * c
+        bound = ref.abs() * (2 * U + (half if g.dtype == BF16 else 0.0))
+        assert ((g.double() - ref).abs() <= bound).all()
+        if share >= 1:
+            assert torch.equal(g, b)
+    assert all(g._version > v for g, v in zip(grads, versions))
+    for t, s in slabs.items():                                                # what lies around the views is as it was
+        assert (s[:1] == 7).all() and (s[at[t]:] == 7).all()
+
+
+def test_clip_of_norms_that_are_not_finite(dev):
+    from denet_amd import ops
+    a, b = torch.ones(300, device=dev), torch.ones(5, device=dev, dtype=BF16)
+    a[7] = math.inf                                                           # coefficient 0: inf * 0 = NaN, the others 0
+    assert float(ops.clip_grads_([a, b], 1.0)) == math.inf
+    assert math.isnan(float(a[7])) and float(a.nan_to_num(0.0).abs().sum()) == 0 and float(b.abs().sum()) == 0
+    a = torch.ones(300, device=dev)
+    a[8] = math.nan
+    assert math.isnan(float(ops.clip_grads_([a], 1.0))) and a.isnan().all()
+
+
+# ---- AdamW: inputs and oracles ---------------------------------------------------------------------------
+def _quant(x, positive):
+    """e4m3 codes and scales, in fp32, of a flat tensor: the format's definition in elementary operations."""
+    n = x.numel()
+    rows = torch.zeros(-(-n // 256) * 256, device=x.device)
+    rows[:n] = x
+    rows = rows.reshape(-1, 256)
+    scale = (torch.where(rows.isfinite(), rows.abs(), 0.0).amax(dim=1) * torch.tensor(1 / 448.0, device=x.device)).clamp(min=TINY)
+    y = rows * (1.0 / scale)[:, None]
+    y = torch.where(rows.isfinite(), y, math.nan)
+    if positive:
+        y = torch.where(y > 0, y.clamp(min=2.0 ** -9), y)
+    return y.to(E4M3).reshape(-1)[:n], scale
+
+
+def _dequant(code, scale):
+    return code.float() * scale.repeat_interleave(256)[:code.numel()]
+
+
+def _inputs(sizes, pt, gt, bits, dev, seed, offset=0, fresh=False):
+    g = _gen(dev, seed)
+    rand = lambda n: torch.randn(n, device=dev, generator=g)
+    d = dict(p=[], g=[], m=[], v=[], ms=[], vs=[])
+    for i, n in enumerate(sizes):
+        gs = 10.0 ** (i % 4 - 4)
+        slab = lambda x, t: torch.cat([torch.zeros(offset, device=dev), x]).to(t)[offset:]
+        grad = rand(n) * gs
+        grad[torch.rand(n, device=dev, generator=g) < 0.1] = 0.0
+        m, r = rand(n) * 0.3 * gs, (torch.rand(n, device=dev, generator=g) + 0.05) * gs
+        if fresh or i % 5 == 4:
+            m, r = torch.zeros_like(m), torch.zeros_like(r)
+        d["p"].append(slab(rand(n) * 0.05, pt))
+        d["g"].append(slab(grad, gt))
+        if bits == 8:
+            for k, x in (("m", m), ("v", r)):
+                code, scale = _quant(x, k == "v")
+                d[k].append(torch.cat([torch.zeros(4 * offset, device=dev).to(E4M3).view(torch.uint8), code.view(torch.uint8)])[4 * offset:].view(E4M3))
+                d[k + "s"].append(scale)
+        else:
+            d["m"].append(slab(m, F32))
+            d["v"].append(slab(r.square(), F32))
+    return d
+
+
+def _clone(d):
+    return {k: [t.clone() for t in v] for k, v in d.items()}
+
+
+def _plan(d, bits, **kw):
+    from denet_amd import ops
+    scales = (d["ms"], d["vs"]) if bits == 8 else ()
+    return ops.AdamWPlan(d["p"], d["g"], d["m"], d["v"], *scales, **kw)
+
+
+H = dict(lr=3e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+
+
+def _same(a, b):
+    if a.dtype == E4M3:                                 # bit for bit, but e4m3 has two NaN codes (7f, ff) of one meaning
+        canon = lambda x: torch.where(x.view(torch.uint8) == 255, torch.full_like(x.view(torch.uint8), 127), x.view(torch.uint8))
+        return torch.equal(canon(a), canon(b))
+    return torch.equal(a.nan_to_num(1.5e38), b.nan_to_num(1.5e38))
+
+
+def _same_arithmetic(d, i, t, coef, bits, lr, betas, eps, weight_decay):
+    """Tensor i after step t in fp32, one elementary operation after the other: (p, m, v, ms, vs)."""
+    f = lambda x: torch.tensor(x, dtype=F32, device=d["p"][i].device)
+    b1, b2 = betas
+    g = d["g"][i].float() * f(coef)
+    if bits == 8:
+        m = _dequant(d["m"][i], d["ms"][i])
+        r = _dequant(d["v"][i], d["vs"][i])
+        v = r * r
+    else:
+        m, v = d["m"][i], d["v"][i]
+    m = m * f(b1) + g * f(1 - b1)
+    v = v * f(b2) + (g * g) * f(1 - b2)
+    r = v.sqrt()
+    denom = r * f(1 / math.sqrt(1 - b2 ** t)) + f(eps)
+    p = (d["p"][i].float() * f(1 - lr * weight_decay) - (m / denom) * f(lr / (1 - b1 ** t))).to(d["p"][i].dtype)
+    if bits == 32:
+        return p, m, v, None, None
+    (mc, ms), (rc, rs) = _quant(m, False), _quant(r, True)
+    return p, mc, rc, ms, rs
+
+
+def _check_64(d, got, i, t, coef, bits, lr, betas, eps, weight_decay):
+    """`got` against the formula in 64 bits, with the bounds counted above."""
+    b1, b2 = betas
+    k = (6, 10) if bits == 8 else (5, 8)
+    g = d["g"][i].double() * coef
+    if bits == 8:
+        sc = lambda x: x.double().repeat_interleave(256)[:g.numel()]
+        m0, v0 = d["m"][i].double() * sc(d["ms"][i]), (d["v"][i].double() * sc(d["vs"][i])) ** 2
+    else:
+        m0, v0 = d["m"][i].double(), d["v"][i].double()
+    m, v = m0 * b1 + g * (1 - b1), v0 * b2 + g * g * (1 - b2)
+    em = k[0] * U * ((m0 * b1).abs() + (g * (1 - b1)).abs()) + 2.0 ** -148
+    r = v.sqrt()
+    er = (k[1] / 2 + 1) * U * r + 2.0 ** -75        # (a square that underflows: sqrt(2^-149))
+    denom = r / math.sqrt(1 - b2 ** t) + eps
+    S, p0 = lr / (1 - b1 ** t), d["p"][i].double()
+    p = p0 * (1 - lr * weight_decay) - S * m / denom
+    ed = (er / math.sqrt(1 - b2 ** t)) / denom + 4 * U
+    ep = 2 * U * p0.abs() + S * (em / denom * 1.01 + (m / denom).abs() * (ed + 3 * U)) + U * p.abs()
+    ep = ep * 1.001 + (2.0 ** -8 * p.abs() if got["p"][i].dtype == BF16 else 0.0)
+    assert ((got["p"][i].double() - p).abs() <= ep).all()
+    if bits == 32:
+        assert ((got["m"][i].double() - m).abs() <= em).all()
+        assert ((got["v"][i].double() - v).abs() <= 8.01 * U * v + 2.0 ** -148).all()
+        return
+    for key, x, ex in (("m", m, em), ("v", r, er)):
+        n = x.numel()
+        pad = torch.zeros(-(-n // 256) * 256 - n, dtype=torch.float64, device=x.device)
+        rows, errs = torch.cat([x.abs(), pad]).reshape(-1, 256), torch.cat([ex.expand_as(x), pad]).reshape(-1, 256)
+        s = got[key + "s"][i].double()
+        want = (rows.amax(dim=1) / 448).clamp(min=TINY)
+        assert ((s - want).abs() <= errs.amax(dim=1) / 448 + 4 * U * want).all()
+        s = s.repeat_interleave(256)[:n]
+        y = x.abs() / s
+        # half a step of e4m3: 2^-4 of the value, 2^-10 below 2^-6; sqrt(v) > 0 is moved up to 2^-9 at most
+        half = torch.maximum(y * 2.0 ** -4, torch.full_like(y, 2.0 ** -10))
+        if key == "v":
+            half = torch.where(y < 2.0 ** -9, torch.full_like(y, 2.0 ** -9), half)
+            assert ((got["v"][i].double() > 0) | (x <= 2.0 ** -74)).all()
+        assert ((got[key][i].double() * s - x).abs() <= s * half * (1 + 1e-5) + ex + 8 * U * x.abs()).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("pt,gt", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("sizes,offset", [([1], 0), (SIZES, 0), (SIZES, 1), ([5, 300] * 60, 3), ([1_500_013], 1)])
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_one_step(bits, pt, gt, sizes, offset, clip, dev):
+    d = _inputs(sizes, pt, gt, bits, dev, 3, offset)
+    got = _clone(d) if offset == 0 else {k: list(v) for k, v in d.items()}
+    if offset:                                          # odd addresses: the views themselves are stepped, copies are the oracle's
+        d = _clone(d)
+    norm64 = _norm64(d["g"])
+    limit = 0.3 * norm64
+    coef = min(1.0, limit / (norm64 + 1e-6)) if clip else 1.0
+    t = 7
+    versions = [p._version for p in got["p"]]
+    norm = _plan(got, bits).step(t, max_norm=limit if clip else None, **H)
+    assert all(p._version > v for p, v in zip(got["p"], versions))
+    if clip:
+        assert abs(float(norm) - norm64) <= 1.01 * U * norm64
+    else:
+        assert norm is None
+    for i in range(len(sizes)):
+        assert torch.equal(got["g"][i], d["g"][i])
+        for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, i, t, coef, bits, **H)):
+            if want is not None:
+                assert _same(got[key][i], want), (key, i, sizes[i])
+        _check_64(d, got, i, t, coef, bits, **H)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("hyper", [dict(H, weight_decay=0.0), dict(H, betas=(0.0, 0.0)), dict(H, betas=(0.0, 0.99)), dict(H, eps=1e-3),
+                                   dict(H, lr=0.0), dict(H, lr=2.0, weight_decay=0.5)])
+@pytest.mark.parametrize("t", [1, 2, 1000, 10 ** 7])
+def test_adamw_hyperparameters(bits, hyper, t, dev):
+    sizes = [1000, 77]
+    d = _inputs(sizes, F32, F32, bits, dev, 4, fresh=t == 1)
+    got = _clone(d)
+    _plan(got, bits).step(t, **hyper)
+    for i in range(2):
+        for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, i, t, 1.0, bits, **hyper)):
+            if want is not None:
+                assert _same(got[key][i], want), (key, i)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps_of_their_own(bits, dev):
+    sizes, steps = [1000, 77, 256], [1, 5, 100000]
+    d = _inputs(sizes, F32, F32, bits, dev, 5)
+    got = _clone(d)
+    plan = _plan(got, bits)
+    plan.step(steps, **H)
+    for i, t in enumerate(steps):
+        for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, i, t, 1.0, bits, **H)):
+            assert want is None or _same(got[key][i], want)
+    d = _clone(got)
+    plan.step(9, **H)                                   # and one number for all again
+    assert _same(got["p"][1], _same_arithmetic(d, 1, 9, 1.0, bits, **H)[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_around_the_tensors_is_touched(bits, dev):
+    """States, scales and parameters as slices of slabs whose other bytes hold a pattern."""
+    n, pad = 1003, 64
+    d = _inputs([n], F32, F32, bits, dev, 6)
+    slabs = {}
+    for k, v in d.items():
+        if not v:
+            continue
+        raw = torch.full((pad * 4 + v[0].nbytes + pad * 4 + 4,), 0x5a, dtype=torch.uint8, device=dev)
+        mid = raw[pad * 4:pad * 4 + v[0].nbytes]
+        mid.copy_(v[0].view(torch.uint8))
+        slabs[k] = (raw, v[0].nbytes)
+        d[k] = [mid.view(v[0].dtype)]
+    before = _clone(d)
+    _plan(d, bits).step(3, max_norm=0.01, **H)
+    for k, (raw, nbytes) in slabs.items():
+        assert (raw[:pad * 4] == 0x5a).all() and (raw[pad * 4 + nbytes:] == 0x5a).all(), k
+        assert k == "g" or not torch.equal(before[k][0].view(torch.uint8), d[k][0].view(torch.uint8)), k
+    assert torch.equal(d["g"][0], before["g"][0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_values_that_are_not_finite_stay_where_they_are(bits, dev):
+    d = _inputs([1024, 300], F32, F32, bits, dev, 7)
+    d["g"][0][300] = math.nan
+    d["g"][0][301] = math.inf
+    d["g"][0][302] = -math.inf
+    d["g"][1][0] = 1e30                                 # its square overflows fp32: v is infinite, the update 0
+    d["g"][1][299] = 1e-30                              # its square underflows
+    got = _clone(d)
+    plan = _plan(got, bits)
+    plan.step(2, **H)
+    for i in range(2):
+        for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, i, 2, 1.0, bits, **H)):
+            assert want is None or _same(got[key][i], want), (key, i)
+    bad = torch.zeros(1024, dtype=torch.bool, device=dev)
+    bad[300:303] = True
+    assert got["p"][0][bad].isnan().all() and got["p"][0][~bad].isfinite().all()
+    assert got["m"][0].float()[~bad].isfinite().all()
+    plan.step(3, **H)                                   # the next step still leaves the neighbours alone
+    assert got["p"][0][bad].isnan().all() and got["p"][0][~bad].isfinite().all()
+
+
+def test_every_code_is_read_and_every_rounding_is_to_nearest(dev):
+    # all 256 codes as m (sqrt(v): the 127 that are not negative), betas that keep them, no gradient: codes and scales reproduce themselves
+    codes = torch.arange(256, device=dev, dtype=torch.uint8)
+    codes[127], codes[255] = 0, 0                       # (not the two NaNs)
+    one = torch.ones(1, device=dev)
+    d = dict(p=[torch.zeros(256, device=dev)], g=[torch.zeros(256, device=dev)], m=[codes.clone().view(E4M3)],
+             v=[(codes & 127).view(E4M3).clone()], ms=[one.clone()], vs=[one.clone()])
+    got = _clone(d)
+    _plan(got, 8).step(1, lr=1.0, betas=(0.5, 0.75), eps=1e-8, weight_decay=0.0)
+    # m' = m / 2: same codes, half the scale; r' = sqrt(3)/2 r to 2 u: same codes away from ties, of which there are none
+    assert torch.equal(got["m"][0].view(torch.uint8) & 127, codes & 127) and float(got["ms"][0]) == 0.5
+    assert torch.equal(got["v"][0].view(torch.uint8), codes & 127)
+    # a dense sweep of gradients through the quantiser: every rounding equals torch's cast of the same quotient
+    g = torch.cat([torch.linspace(-1, 1, 200001, device=dev), torch.logspace(-8, 0, 100000, device=dev)])
+    z = torch.zeros_like(g)
+    blocks = -(-g.numel() // 256)
+    d = dict(p=[z.clone()], g=[g], m=[z.to(E4M3)], v=[z.to(E4M3)], ms=[torch.zeros(blocks, device=dev)], vs=[torch.zeros(blocks, device=dev)])
+    got = _clone(d)
+    _plan(got, 8).step(1, **H)
+    for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, 0, 1, 1.0, 8, **H)):
+        assert _same(got[key][0], want), key
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_steps(bits, dev):
+    """Forty updates, a new gradient each: bit for bit the fp32 arithmetic; 32-bit states also near 64 bits."""
+    sizes = [777, 256 * 9]
+    d = _inputs(sizes, F32, F32, bits, dev, 8, fresh=True)
+    got = _clone(d)
+    plan = _plan(got, bits)
+    p64, m64, v64 = [[x.double() for x in d["p"]]] + [[torch.zeros_like(x, dtype=torch.float64) for x in d["p"]] for _ in range(2)]
+    gen = _gen(dev, 9)
+    for t in range(1, 41):
+        for i, n in enumerate(sizes):
+            g = torch.randn(n, device=dev, generator=gen) * 0.01
+            d["g"][i].copy_(g)
+            got["g"][i].copy_(g)
+            new = _same_arithmetic(d, i, t, 1.0, bits, **H)
+            for key, x in zip(("p", "m", "v", "ms", "vs"), new):
+                if x is not None:
+                    d[key][i].copy_(x)
+            b1, b2 = H["betas"]
+            m64[i] = m64[i] * b1 + g.double() * (1 - b1)
+            v64[i] = v64[i] * b2 + g.double() ** 2 * (1 - b2)
+            p64[i] = p64[i] * (1 - H["lr"] * H["weight_decay"]) - H["lr"] / (1 - b1 ** t) * m64[i] / (v64[i].sqrt() / math.sqrt(1 - b2 ** t) + H["eps"])
+        plan.step(t, **H)
+    for i in range(2):
+        assert all(_same(got[k][i], d[k][i]) for k in d if d[k])
+        if bits == 32:
+            # an error of e in m or v fades with the moments: at most 10 steps of 5 u (m) and 1000 of 8 u (v, t of them); per step p
+            # gains 2 u |p| + S (quotient error) with |m/d| <= 1 / sqrt(1 - b2)-free bound of Adam's ratio, here <= 10
+            bound = 40 * (4 * U * (p64[i].abs() + 0.2) + H["lr"] * 10 * (50 + 8 * 40) * U)
+            assert ((got["p"][i].double() - p64[i]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_memory_orders(bits, dev):
+    """Channels-last weights: any dense order, the same for a parameter's tensors; others are refused."""
+    from denet_amd import _lib, ops
+    g = _gen(dev, 10)
+    w = torch.randn(24, 16, 3, 3, device=dev, generator=g)
+    flat = _inputs([w.numel()], F32, F32, bits, dev, 11)
+    cl = lambda x: x.as_strided(w.shape, w.to(memory_format=torch.channels_last).stride())
+    d = {k: [cl(x) for x in v] if k in ("p", "g", "m", "v") else v for k, v in _clone(flat).items()}
+    _plan(d, bits).step(2, **H)
+    _plan(flat, bits).step(2, **H)
+    assert _same(d["p"][0], cl(flat["p"][0])) and _same(d["m"][0], cl(flat["m"][0]))
+    with pytest.raises(_lib.DenetHipError):
+        _plan(dict(d, g=[d["g"][0].contiguous()]), bits)
+    with pytest.raises(_lib.DenetHipError):
+        _plan(dict(flat, p=[torch.zeros(2 * w.numel(), device=dev)[::2]]), bits)
+    with pytest.raises(_lib.DenetHipError):
+        ops.GradNormPlan([torch.zeros(8, device=dev)[::2]])
+
+
+def test_refusals(dev):
+    from denet_amd import _lib, ops
+    E = _lib.DenetHipError
+    d, e = _inputs([100, 300], F32, F32, 32, dev, 12), _inputs([100, 300], F32, F32, 8, dev, 12)
+    bad32 = [dict(d, p=[d["p"][0], d["p"][0][:100]]), dict(d, p=[d["p"][0].double(), d["p"][1]]), dict(d, g=[d["g"][0].half(), d["g"][1]]),
+             dict(d, m=[d["m"][0].to(BF16), d["m"][1]]), dict(d, g=d["g"][:1]), dict(d, g=[d["g"][0][:99], d["g"][1]]),
+             dict(d, v=[d["m"][0], d["v"][1]]), dict(d, g=[d["p"][0], d["g"][1]]), dict(d, p=[d["p"][0].cpu(), d["p"][1]]),
+             dict(d, p=[d["p"][0], d["p"][0]], g=[d["g"][0], d["g"][0]], m=[d["m"][0], d["m"][0].clone()], v=[d["v"][0], d["v"][0].clone()])]
+    for x in bad32:
+        with pytest.raises(E):
+            _plan(x, 32)
+    bad8 = [dict(e, ms=[e["ms"][0], e["ms"][1][:1]]), dict(e, vs=[e["vs"][0].double(), e["vs"][1]]), dict(e, m=[d["m"][0], d["m"][1]]),
+            dict(e, m=[torch.zeros(101, dtype=torch.uint8, device=dev)[1:].view(E4M3), e["m"][1]]),
+            dict(e, v=[e["v"][0].view(torch.uint8), e["v"][1]])]
+    for x in bad8:
+        with pytest.raises(E):
+            _plan(x, 8)
+    plan = _plan(d, 32)
+    for kw in (dict(step=0), dict(step=-3), dict(step=None), dict(step=[1]), dict(step=[1, 0]), dict(step=1, lr=-1.0), dict(step=1, betas=(1.0, 0.9)),
+               dict(step=1, eps=-1.0), dict(step=1, max_norm=-1.0), dict(step=1, max_norm=math.nan), dict(step=1, lr=torch.ones((), device=dev)),
+               dict(step=1, coef=torch.ones((), device=dev), max_norm=1.0), dict(step=1, coef=torch.ones(2, device=dev)),
+               dict(step=1, coef=torch.ones(()))):
+        before = d["p"][0].clone()
+        with pytest.raises(E):
+            plan.step(**kw)
+        assert torch.equal(d["p"][0], before)
+    for m in (-1.0, math.nan):
+        with pytest.raises(E):
+            ops.clip_grads_(d["g"], m)
+    with pytest.raises(E):
+        ops.clip_grads_([d["g"][0], d["g"][0]], 1.0)                          # scaled twice
+    assert float(ops.grad_norm([d["g"][0], d["g"][0]])) > 0                   # (only read: allowed)
+    counters = [torch.zeros((), dtype=torch.int64, device=dev) for _ in range(2)]
+    with pytest.raises(E):
+        _plan(d, 32, steps=counters[:1])
+    with pytest.raises(E):
+        _plan(d, 32, steps=[counters[0], counters[0]])
+    with pytest.raises(E):
+        _plan(d, 32, steps=[c.int() for c in counters])
+    with pytest.raises(E):
+        _plan(d, 32, steps=counters).step(1, **H)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_device_counters(bits, dev):
+    n = [333] * 5 + [0] + [70] * 300                    # counters of more than one launch, an empty tensor among them
+    d = _inputs(n, F32, F32, bits, dev, 13)
+    got = _clone(d)
+    steps = [torch.full((), i % 3, dtype=torch.int64, device=dev) for i in range(len(n))]
+    lr = torch.full((1,), H["lr"], device=dev)
+    plan = _plan(got, bits, steps=steps)
+    plan.step(**dict(H, lr=lr))
+    lr32 = float(lr)
+    for i in range(len(n)):
+        if not n[i]:
+            continue
+        assert int(steps[i]) == i % 3 + 1
+        b1, b2 = H["betas"]
+        want = _same_arithmetic(d, i, i % 3 + 1, 1.0, bits, **dict(H, lr=lr32))
+        # the device's pow may differ from the host's in its last bit of 64: the fp32 constants agree but for ties
+        assert _same(got["p"][i], want[0]) and _same(got["m"][i], want[1]) and _same(got["v"][i], want[2])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_replays_equal_eager_steps(bits, dev):
+    sizes = [5, 4097, 70003] + [19] * 70
+    a = _inputs(sizes, F32, BF16, bits, dev, 14, fresh=True)
+    b = _clone(a)
+    steps = [[torch.zeros((), dtype=torch.int64, device=dev) for _ in sizes] for _ in range(2)]
+    lr = torch.full((), 1e-3, device=dev)
+    pa, pb = _plan(a, bits, steps=steps[0]), _plan(b, bits, steps=steps[1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        na = pa.step(**dict(H, lr=lr), max_norm=0.05)   # one eager step of both
+        nb = pb.step(**dict(H, lr=lr), max_norm=0.05)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        na = pa.step(**dict(H, lr=lr), max_norm=0.05)
+    g = _gen(dev, 15)
+    for k in range(6):
+        for i, n in enumerate(sizes):
+            x = torch.randn(n, device=dev, generator=g) * 10.0 ** (-k)
+            a["g"][i].copy_(x)
+            b["g"][i].copy_(x)
+        lr.fill_(1e-3 / (k + 1))
+        graph.replay()
+        nb = pb.step(**dict(H, lr=lr), max_norm=0.05)
+        if k % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(na, nb), k
+        for key in a:
+            assert all(_same(x, y) for x, y in zip(a[key], b[key])), (k, key)
+    assert int(steps[0][0]) == 7 == int(steps[1][-1])
+    host = _plan(_clone(a), bits)
+    with pytest.raises(Exception, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            host.step(1, **H)
+
+
+def test_clip_in_a_graph(dev):
+    from denet_amd import ops
+    grads, _, _ = _grads(SIZES, [F32, BF16], dev, 16, 1)
+    first = [g.clone() for g in grads]
+    plan = ops.GradNormPlan(grads)
+    plan.clip_(1e9)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = plan.clip_(0.5)
+    for k in range(4):
+        for g, f in zip(grads, first):
+            g.copy_(f * (k + 1))
+        ref = [g.clone() for g in grads]
+        want = ops.clip_grads_(ref, 0.5)
+        graph.replay()
+        assert torch.equal(norm, want) and all(torch.equal(x, y) for x, y in zip(grads, ref))
+
+
+def test_streams(dev):
+    """The same plan on other streams than its tensors' own, the workspace of a call reused by the next work of its stream."""
+    d = _inputs([300_001], F32, F32, 32, dev, 17)
+    got, other = _clone(d), _clone(d)
+    plan = _plan(got, 32)
+    for t in range(1, 7):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            norm = plan.step(t, max_norm=0.1, **H)
+            torch.full((4096,), 1e9, device=dev)                              # takes the freed workspace's place, in stream order
+        torch.cuda.current_stream().wait_stream(s)
+    plan2 = _plan(other, 32)
+    for t in range(1, 7):
+        norm2 = plan2.step(t, max_norm=0.1, **H)
+    assert torch.equal(norm, norm2) and torch.equal(got["p"][0], other["p"][0]) and torch.equal(got["v"][0], other["v"][0])
+
+
+def test_long_tensor(dev):
+    """Element offsets beyond 2^31 (bytes beyond 2^33): the last elements of a long tensor are stepped and counted."""
+    from denet_amd import ops
+    n = 2 ** 31 + 4099
+    g = torch.zeros(n, dtype=BF16, device=dev)
+    g[-3:] = 2.0
+    g[2 ** 31 - 1] = 1.0
+    assert abs(float(ops.grad_norm([g])) - math.sqrt(13.0)) <= 1.01 * U * math.sqrt(13.0)
+    ops.clip_grads_([g], math.sqrt(13.0) / 2 + 5e-7)
+    assert float(g[-1]) == 1.0 and float(g[2 ** 31 - 1]) == 0.5
+    p = torch.zeros(n, dtype=BF16, device=dev)
+    codes = [torch.zeros(n, dtype=torch.uint8, device=dev).view(E4M3) for _ in range(2)]
+    scales = [torch.zeros(-(-n // 256), device=dev) for _ in range(2)]
+    ops.adamw_step([p], [g], codes[:1], codes[1:], 1, scales[:1], scales[1:], lr=0.5, weight_decay=0.0)
+    # the first step is lr * sign(g) (eps is far below |g|)
+    assert float(p[-1]) == -0.5 and float(p[2 ** 31 - 1]) == -0.5 and float(p[2 ** 31]) == 0.0 and float(p[12345]) == 0.0
+    assert float(codes[0][-1].float()) == 448.0 and float(codes[1][2 ** 31 - 1].float()) == 448.0
+    tail = scales[0][-1].double() * 448
+    assert abs(float(tail) - 0.1) <= 8 * U
+
+
+# ---- the optimizer ------------------------------------------------------------------------------------------
+def _model(dev, seed=0):
+    torch.manual_seed(seed)
+    m = torch.nn.Sequential(torch.nn.Conv2d(3, 10, 3), torch.nn.BatchNorm2d(10), torch.nn.ReLU(), torch.nn.Conv2d(10, 5, 1)).to(dev)
+    m[0] = m[0].to(memory_format=torch.channels_last)
+    return m
+
+
+def _set_grads(models, seed, dev, scale=1.0):
+    g = _gen(dev, seed)
+    for ps in zip(*(m.parameters() for m in models)):
+        x = torch.randn(ps[0].shape, device=dev, generator=g) * scale
+        for p in ps:
+            p.grad = x.clone()                          # contiguous, also where the parameter is channels-last
+
+
+def test_optimizer_against_torch(dev):
+    """32-bit states: within rounding of torch.optim.AdamW and clip_grad_norm_ over ten steps, groups with settings of their own, a parameter
+    whose gradient is missing now and then."""
+    from denet_amd.optim import AdamW
+    a, b = _model(dev), _model(dev)
+    groups = lambda m: [dict(params=list(m[0].parameters()), lr=2e-3), dict(params=[*m[1].parameters(), *m[3].parameters()], weight_decay=0.1, betas=(0.8, 0.95))]
+    ours, ref = AdamW(groups(a), lr=1e-3, max_norm=0.7), torch.optim.AdamW(groups(b), lr=1e-3)
+    for t in range(10):
+        _set_grads((a, b), 20 + t, dev, 0.1 * (t + 1))
+        if t % 3 == 1:
+            a[3].bias.grad = b[3].bias.grad = None
+        norm = torch.nn.utils.clip_grad_norm_(b.parameters(), 0.7)
+        kept = [p.grad.clone() if p.grad is not None else None for p in a.parameters()]
+        ours.step()
+        ref.step()
+        assert abs(float(ours.grad_norm) - float(norm)) <= 1e-5 * float(norm)
+        assert all(k is None or torch.equal(k, p.grad) for k, p in zip(kept, a.parameters()))
+    for p, q in zip(a.parameters(), b.parameters()):
+        # both are fp32 evaluations of one formula: per step a few u of |p| and of lr * |m/d| (<= 10) apart
+        assert ((p - q).abs() <= 10 * (8 * U * q.abs() + 3e-3 * 10 * 60 * U)).all()
+    assert ours.state[a[3].bias]["step"] == 7 and ours.state[a[0].weight]["step"] == 10
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_optimizer_checkpoint(bits, capturable, dev, tmp_path):
+    from denet_amd.optim import AdamW
+    a, b = _model(dev), _model(dev, 1)
+    mk = lambda m: AdamW(m.parameters(), lr=1e-2, state_bits=bits, max_norm=1.0, capturable=capturable)
+    oa, ob = mk(a), mk(b)
+    for t in range(3):
+        _set_grads((a,), 30 + t, dev)
+        oa.step()
+    torch.save({"m": a.state_dict(), "o": oa.state_dict()}, tmp_path / "c.bin")
+    d = torch.load(tmp_path / "c.bin", map_location=dev, weights_only=True)
+    b[0] = b[0].to(memory_format=torch.channels_last)
+    b.load_state_dict(d["m"])
+    ob.load_state_dict(d["o"])
+    for t in range(3):
+        _set_grads((a, b), 40 + t, dev)
+        oa.step()
+        ob.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q)
+        for k, v in oa.state[p].items():
+            w = ob.state[q][k]
+            assert int(v) == int(w) == 6 if k == "step" else (v.dtype == w.dtype and _same(v, w))
+    p = next(iter(a.parameters()))
+    n = sum(v.nbytes for k, v in oa.state[p].items() if k != "step")
+    assert n == (2 * p.numel() + 8 * -(-p.numel() // 256) if bits == 8 else 8 * p.numel())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_in_a_graph(bits, dev):
+    """Forward, backward and step captured together, against eager steps; the eager optimizer refuses the capture."""
+    from denet_amd.optim import AdamW
+    w0 = torch.randn(64, 32, device=dev, generator=_gen(dev, 50))
+    x = torch.randn(16, 32, device=dev, generator=_gen(dev, 51))
+    a, b = torch.nn.Parameter(w0.clone()), torch.nn.Parameter(w0.clone())
+    lr = torch.full((), 1e-2, device=dev)
+    oa, ob = (AdamW([p], lr=lr, state_bits=bits, max_norm=0.5, capturable=True) for p in (a, b))
+    grad = lambda p: ((x @ p.detach().t()).tanh().t() @ x).mul_(0.1)
+    a.grad, b.grad = grad(a), grad(b)
+    oa.step()
+    ob.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.grad.copy_(grad(a))
+        oa.step()
+    for k in range(5):
+        lr.fill_(1e-2 / (k + 1))
+        graph.replay()
+        b.grad.copy_(grad(b))
+        ob.step()
+        torch.cuda.synchronize()
+        # (library products in and out of a graph: compared after the same number of updates of the same algorithm)
+        assert torch.equal(a, b), k
+    with pytest.raises(Exception, match="capturable"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            c = AdamW([b])
+            c.step()
+
+
+def test_versions_are_seen_by_autograd(dev):
+    from denet_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    y = (p * p).sum()
+    p.grad = torch.ones(8, device=dev)
+    AdamW([p]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_gradients_in_other_forms(dev):
+    from denet_amd import _lib
+    from denet_amd.optim import AdamW, clip_grad_norm_
+    p, q = (torch.nn.Parameter(torch.ones(6, 4, device=dev)) for _ in range(2))
+    p.grad = torch.ones(4, 1, device=dev).t().expand(6, 4)                    # a broadcast gradient: no memory of its own per element
+    q.grad = torch.ones(6, 4, device=dev)
+    AdamW([p]).step()
+    AdamW([q]).step()
+    assert torch.equal(p, q)
+    p.grad = None
+    p.grad = torch.ones(6, 4, device=dev).to_sparse()
+    with pytest.raises(_lib.DenetHipError):
+        AdamW([p]).step()
+    q.grad = torch.full((6, 4), math.nan, device=dev)
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([q], 1.0, error_if_nonfinite=True)
+    r = torch.nn.Parameter(torch.zeros(0, device=dev))
+    r.grad = torch.zeros(0, device=dev)
+    AdamW([r], max_norm=1.0).step()
+
+
+# ---- the trainer ----------------------------------------------------------------------------------------------
+def _trainer(tmp_path, optimizer, **train):
+    from denet_amd.trainer import DENetTrainer
+    torch.manual_seed(0)
+    return DENetTrainer({
+        "model": {"arch": "DENet", "backbone": "synthetic", "maximum_num_classes": 21},
+        "data": {"train_dataset": "synthetic", "val_dataset": "synthetic", "img_size": 65, "shot": 2, "batch_size": 4, "batches_per_epoch": 2,
+                 "val_batches": 1},
+        "train": dict({"trainer": "DENetTrainer", "device": 0, "num_steps": 3, "log_steps": 100, "val_steps": 2, "logdir": str(tmp_path),
+                       "optimizer": optimizer, "loss": {"name": "loss_denet"}}, **train)})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_trainer_with_fused_adamw(bits, dev, tmp_path):
+    """train.optimizer.name: fused_adamw with train.max_grad_norm: after two steps the parameters are what the formula in the same arithmetic makes
+    of the gradients that the trainer's bucket held; the training loop runs and its checkpoint holds the states."""
+    tr = _trainer(tmp_path, dict(name="fused_adamw", lr=1e-3, weight_decay=0.01, state_bits=bits), max_grad_norm=0.05)
+    params = [p for p in tr.model.parameters() if p.requires_grad]
+    assert len(params) == 24
+    for t in (1, 2):
+        d = dict(p=[p.detach().reshape(-1).clone() for p in params], g=[], m=[], v=[], ms=[], vs=[])
+        for p in params:
+            st, n = tr.optimizer.state[p], p.numel()
+            for key, name in (("m", "exp_avg"), ("v", "exp_avg_sqrt" if bits == 8 else "exp_avg_sq")):
+                z = torch.zeros(n, device=dev)
+                d[key].append(st[name].reshape(-1).clone() if st else z.to(E4M3) if bits == 8 else z)
+                d[key + "s"].append(None if bits == 32 else st[name + "_scale"].clone() if st else torch.zeros(-(-n // 256), device=dev))
+        tr.step(tr.train_loader.batch(t), train=True)
+        d["g"] = [p.grad.reshape(-1) for p in params]
+        norm = _norm64(d["g"])
+        assert abs(float(tr.grad_norm) - norm) <= 1.01 * U * norm and norm > 0.05
+        for i, p in enumerate(params):
+            want = _same_arithmetic(d, i, t, 0.05 / (norm + 1e-6), bits, 1e-3, (0.9, 0.999), 1e-8, 0.01)
+            assert _same(p.detach().reshape(-1), want[0]) and _same(tr.optimizer.state[p]["exp_avg"].reshape(-1), want[1]), (t, i)
+    tr.train()
+    d = torch.load(str(tmp_path / "latest_model.bin"), weights_only=True)
+    assert d["optimizer"]["state"][0]["exp_avg"].dtype == (E4M3 if bits == 8 else F32)
+    tr.optimizer.load_state_dict(d["optimizer"])
+
+
+def test_trainer_clips_for_any_optimizer(dev, tmp_path):
+    tr = _trainer(tmp_path, dict(name="sgd", lr=0.1), max_grad_norm=0.01)
+    params = [p for p in tr.model.parameters() if p.requires_grad]
+    before = [p.detach().clone() for p in params]
+    tr.step(tr.train_loader.batch(0), train=True)
+    assert float(tr.grad_norm) > 0.01
+    assert abs(_norm64([tr.bucket.flat]) - 0.01) <= 0.01 * (2e-6 / 0.01 + 4 * U)
+    for p, b in zip(params, before):
+        assert ((p.detach() - (b.double() - 0.1 * p.grad.double())).abs() <= 3 * U * (b.abs() + 0.1 * p.grad.abs())).all()
+    plain = _trainer(tmp_path, dict(name="sgd", lr=0.1))
+    plain.step(plain.train_loader.batch(0), train=True)
+    assert plain.grad_norm is None

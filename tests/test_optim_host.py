@@ -1,0 +1,177 @@
+"""CPU: refusals of the optimizer operators (nothing of these reaches a GPU)."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _row(_lib, **kw):
+    """One denet_opt_tensor_t as words; made-up, suitably aligned addresses (never dereferenced on the host)."""
+    d = dict(param=0x10000, grad=0x20000, m=0x30000, v=0x40000, ms=0x50000, vs=0x60000, n=1000, step=1, step_dev=0, pt=0, gt=0)
+    d.update(kw)
+    return [d["param"], d["grad"], d["m"], d["v"], d["ms"], d["vs"], d["n"], d["step"], d["step_dev"], d["pt"] | (d["gt"] << 32)]
+
+
+def _table(rows):
+    flat = [w for r in rows for w in r]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _hyper(_lib, **kw):
+    h = _lib.AdamWHyper()
+    d = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, max_norm=-1.0, device_steps=0)
+    d.update(kw)
+    for k, v in d.items():
+        setattr(h, k, v)
+    return h
+
+
+BADARG, UNSUPPORTED, WORKSPACE = -1, -2, -4
+WS, NORM = 0x70000, 0x80000
+
+
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(grad=0), dict(grad=0x20002), dict(grad=0x20001, gt=1), dict(gt=2), dict(n=1 << 48)])
+def test_abi_refuses_bad_gradients(bad):
+    from denet_amd import _lib
+    lib = _lib.load()
+    t = _table([_row(_lib), _row(_lib, **bad)])
+    need = _lib.query("denet_opt_workspace", 2)
+    assert lib.denet_grad_norm(ctypes.addressof(t), 2, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_clip(ctypes.addressof(t), 2, 1.0, NORM, WS, need, None) == BADARG
+    h = _hyper(_lib)
+    assert lib.denet_adamw_step(ctypes.addressof(t), 2, 32, ctypes.addressof(h), None, None, 0, None) == BADARG
+
+
+def test_abi_refuses_bad_calls():
+    from denet_amd import _lib
+    lib = _lib.load()
+    t = _table([_row(_lib)])
+    a, need = ctypes.addressof(t), _lib.query("denet_opt_workspace", 1)
+    assert lib.denet_grad_norm(a, -1, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(None, 1, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, -1.0, None, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, -1.0, NORM, NORM, WS, need, None) == BADARG            # a coefficient needs max_norm
+    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, None, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, WS + 4, need, None) == BADARG        # workspace alignment
+    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, WS, need - 1, None) == WORKSPACE
+    for m in (-1.0, float("nan")):
+        assert lib.denet_grad_clip(a, 1, m, NORM, WS, need, None) == BADARG
+    assert _lib.query("denet_opt_workspace", -1) == BADARG
+    assert _lib.query("denet_opt_workspace", 0) > 0
+    huge = _table([_row(_lib, n=(1 << 48) - 1)])                                            # more chunks than a grid has blocks
+    assert lib.denet_grad_norm(ctypes.addressof(huge), 1, -1.0, NORM, None, WS, need, None) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_abi_refuses_bad_steps(bits):
+    from denet_amd import _lib
+    lib = _lib.load()
+    need = _lib.query("denet_opt_workspace", 1)
+
+    def call(row={}, norm=None, ws=None, ws_bytes=0, bits=bits, **hyper):
+        t, h = _table([_row(_lib, **row)]), _hyper(_lib, **hyper)
+        return lib.denet_adamw_step(ctypes.addressof(t), 1, bits, ctypes.addressof(h), norm, ws, ws_bytes, None)
+
+    for row in (dict(param=0), dict(m=0), dict(v=0), dict(param=0x10002), dict(param=0x10001, pt=1), dict(pt=7), dict(step=0), dict(m=0x30002),
+                dict(v=0x40001)):
+        assert call(row) == BADARG, row
+    if bits == 8:
+        assert call(dict(ms=0)) == BADARG and call(dict(vs=0x60002)) == BADARG
+    for hyper in (dict(lr=-1.0), dict(lr=float("nan")), dict(beta1=1.0), dict(beta2=-0.1), dict(beta2=float("nan")), dict(eps=-1e-8),
+                  dict(weight_decay=-0.1), dict(max_norm=float("nan"))):
+        assert call(**hyper) == BADARG, hyper
+    assert call(bits=16) == BADARG
+    assert call(max_norm=1.0, ws=WS, ws_bytes=need) == BADARG                               # no place for the norm
+    assert call(max_norm=1.0, norm=NORM) == BADARG                                          # no workspace
+    assert call(max_norm=1.0, norm=NORM, ws=WS, ws_bytes=need - 1) == WORKSPACE
+    assert call(max_norm=1.0, norm=NORM, ws=WS, ws_bytes=need, coef=NORM) == BADARG         # both kinds of clipping
+    assert call(lr_dev=NORM) == BADARG                                                      # lr on the device without counters there
+    assert call(device_steps=1, ws=WS, ws_bytes=need) == BADARG                             # no counter
+    assert call(dict(step_dev=0x90004), device_steps=1, ws=WS, ws_bytes=need) == BADARG
+    assert call(dict(step_dev=0x90000), device_steps=1) == BADARG
+
+
+def test_nothing_to_do_needs_no_gpu():
+    from denet_amd import _lib
+    lib = _lib.load()
+    h = _hyper(_lib)
+    t = _table([_row(_lib, n=0, param=0, grad=0, m=0, v=0, step=0)])
+    assert lib.denet_adamw_step(ctypes.addressof(t), 1, 32, ctypes.addressof(h), None, None, 0, None) == 0
+    assert lib.denet_adamw_step(None, 0, 32, ctypes.addressof(h), None, None, 0, None) == 0
+
+
+def test_plans_refuse_cpu_tensors_and_empty_lists():
+    from denet_amd import _lib, ops
+    x = [torch.zeros(4)]
+    for call in (lambda: ops.GradNormPlan(x), lambda: ops.GradNormPlan([]), lambda: ops.GradNormPlan([1.0]), lambda: ops.grad_norm(x),
+                 lambda: ops.clip_grads_(x, 1.0), lambda: ops.AdamWPlan(x, x, x, x), lambda: ops.AdamWPlan([], [], [], []),
+                 lambda: ops.adamw_step(x, x, x, x, 1), lambda: ops.AdamWPlan(x, [], x, x), lambda: ops.AdamWPlan(x, x, x, x, x)):
+        with pytest.raises(_lib.DenetHipError):
+            call()
+
+
+def test_overlap_is_found():
+    from denet_amd.multi_tensor import _check_overlap, _dense, _spans
+    from denet_amd._lib import DenetHipError
+    x = torch.zeros(100)
+    _check_overlap(_spans([x[:50], x[50:]]), _spans([torch.zeros(5)]))
+    _check_overlap(_spans([x[:50], x[90:]]), _spans([x[50:90]]))
+    for written, read in (([x, x], []), ([x[:51], x[50:]], []), ([x[:50]], [x[49:60]]), ([x[10:20], x[60:70]], [x[:100]]), ([x], [x[7:8]])):
+        with pytest.raises(DenetHipError):
+            _check_overlap(_spans(written), _spans(read))
+    assert _dense(torch.zeros(2, 3, 4, 5).to(memory_format=torch.channels_last)) and _dense(torch.zeros(3, 4).t())
+    assert not _dense(torch.zeros(4, 4)[:, :3]) and not _dense(torch.zeros(4, 1).expand(4, 4)) and not _dense(torch.zeros(8)[::2])
+
+
+def test_optimizer_arguments():
+    from denet_amd.optim import AdamW, clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(betas=(0.9,)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(state_bits=16),
+               dict(lr=torch.tensor(1e-3))):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(Exception):
+        AdamW([p], max_norm=float("nan"))
+    with pytest.raises(ValueError):
+        AdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))])
+    with pytest.raises(Exception):
+        AdamW([torch.nn.Parameter(p.detach()[:3]), torch.nn.Parameter(p.detach()[2:])])     # views of the same elements
+    opt = AdamW([p])
+    opt.step()                                                                              # no gradients: nothing to do
+    assert not opt.state and float(clip_grad_norm_([p], 1.0)) == 0.0
+    p.grad = torch.ones(4)
+    from denet_amd._lib import DenetHipError
+    with pytest.raises(DenetHipError):
+        opt.step()                                                                          # there is no CPU path
+    with pytest.raises(DenetHipError):
+        clip_grad_norm_([p], 1.0)
+
+
+def test_load_state_dict_refuses_other_optimizers():
+    from denet_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([p], state_bits=32)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(torch.optim.SGD([p], lr=0.1, momentum=0.9).state_dict())
+    other = torch.optim.AdamW([p], lr=0.25, betas=(0.8, 0.9), amsgrad=True)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(other.state_dict())
+    other = torch.optim.AdamW([p], lr=0.25, betas=(0.8, 0.9))
+    p.grad = torch.ones(4)
+    other.step()
+    other.step()
+    opt.load_state_dict(other.state_dict())                                                 # stock state: taken over
+    assert opt.param_groups[0]["lr"] == 0.25 and tuple(opt.param_groups[0]["betas"]) == (0.8, 0.9)
+    s, o = opt.state[p], other.state[p]
+    assert s["step"] == 2 and torch.equal(s["exp_avg"], o["exp_avg"]) and torch.equal(s["exp_avg_sq"], o["exp_avg_sq"])
+    assert s["exp_avg"].data_ptr() != o["exp_avg"].data_ptr()
+    with pytest.raises(ValueError):
+        AdamW([p], state_bits=8).load_state_dict(other.state_dict())
+    # and its own state comes back unchanged, types included
+    again = AdamW([p], state_bits=32)
+    again.load_state_dict(opt.state_dict())
+    assert torch.equal(again.state[p]["exp_avg"], s["exp_avg"]) and again.state[p]["step"] == 2
+    half = torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))
+    kept = AdamW([half])
+    kept.load_state_dict(opt.state_dict())
+    assert kept.state[half]["exp_avg"].dtype == torch.float32
