@@ -51,9 +51,10 @@ _SIGS = {
     "denet_head_step_train_fwd": "ppi" "LLLLF" "FFFFFFF" "FF" "h" "lllllllll" "i" "FFF" "pl" "h",
     "denet_head_step_train_bwd": "piL" "FFF" "FF" "h" "F" "lllllllll" "pp" "FFFFFFF" "Fi" "pl" "h",
     "denet_dropout_mask": "uifl" "F",
-    "denet_grad_norm": "ald" "FF" "pl",
-    "denet_grad_clip": "ald" "F" "pl",
-    "denet_adamw_step": "alia" "F" "pl",
+    "denet_opt_table": "al" "pl",
+    "denet_grad_norm": "alpd" "FF" "pl",
+    "denet_grad_clip": "alpd" "F" "pl",
+    "denet_adamw_step": "alpia" "F" "pl",
 }
 _NOSTREAM = {
     "denet_version": (ctypes.c_char_p, ""),
@@ -65,6 +66,7 @@ _NOSTREAM = {
     "denet_upsample_loss_parts": (ctypes.c_int64, "llllli"),
     "denet_head_step_plan": (ctypes.c_int, "lllllllllih"),
     "denet_opt_workspace": (ctypes.c_int64, "l"),
+    "denet_opt_table_bytes": (ctypes.c_int64, "al"),
 }
 _CT = {"p": ctypes.c_void_p, "F": ctypes.c_void_p, "L": ctypes.c_void_p, "l": ctypes.c_int64, "u": ctypes.c_uint64, "i": ctypes.c_int, "f": ctypes.c_float, "h": ctypes.c_void_p,
        "a": ctypes.c_void_p, "d": ctypes.c_double}

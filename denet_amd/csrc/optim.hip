@@ -1,10 +1,5 @@
 // Optimizer operators over many tensors at once: the global L2 norm of a gradient list (with its clipping form) and the
 // AdamW step with 32-bit or 8-bit states.
-//
-// A call takes a HOST array of tensor descriptors.  They travel as kernel arguments (at most 4 KB), so a launch covers
-// up to OPT_SLOTS tensors and nothing has to be copied to the device first, kept between calls or re-validated: a
-// captured graph holds its own copy.  The work is cut into chunks of CHUNK elements; `start[i]` is the first chunk of
-// tensor i in the launch, and a block finds its tensor with one vector load and a ballot over the starts.
 #include <math.h>
 #include "denet_common.hpp"
 
@@ -12,9 +7,17 @@
 #pragma clang fp contract(off)
 
 #define OPT_THREADS 256
-#define OPT_SLOTS 64                // one lane per tensor in the look-up
-#define QBLOCK 256                  // consecutive elements that share a scale of the 8-bit states (one wave, 4 per lane)
+#ifndef OPT_U
+#define OPT_U 1
+#endif
+#define OPT_CHUNK (4 * OPT_U * OPT_THREADS)   // elements of a block: OPT_U vectors of four for each thread
+#define QBLOCK DENET_OPT_QBLOCK     // consecutive elements that share a scale of the 8-bit states (one wave, 4 per lane)
+#ifndef NORM_PARTS
 #define NORM_PARTS 1024             // most partial sums of a norm: every block of the consumer adds them up itself
+#endif
+#ifndef NORM_LEAST
+#define NORM_LEAST 4                // least chunks of a block of the norm
+#endif
 #define E4M3_MAX 448.f
 #define SCALE_MIN 1.1754943508222875e-38f   // 2^-126
 
@@ -65,26 +68,43 @@ __device__ __forceinline__ KARG(T)* kernel_args() {
     return (KARG(T)*)__builtin_amdgcn_kernarg_segment_ptr();
 }
 
-// the tensor that chunk `b` of a launch belongs to; starts[count..63] are not read into the vote
-__device__ __forceinline__ int find_slot(KARG(int)* starts, int count, int b) {
+// ---- the list of tensors -------------------------------------------------------------------------------------------
+// A list is cut into chunks of OPT_CHUNK elements; chunk b of a launch belongs to one tensor.  Two forms:
+//  - Packed: the descriptors are kernel arguments.  `start[i]` is the first chunk of tensor i in the launch; a block finds its
+//    tensor with one load by its lanes and a ballot.  At most PACK tensors a launch.
+//  - Tabled: descriptors and the owner of every chunk lie in device memory (written once by denet_opt_table): any
+//    number of tensors in one launch, no search.
+struct Slot {
+    void* p; void* g; void* m; void* v; float* ms; float* vs;
+    int64_t n;                       // bits 0..47 elements, bit 60: bf16 parameter, bit 61: bf16 gradient
+    int start;                       // first chunk
+    int index;                       // in the caller's list (its place in the clock)
+};
+#define PACK 52                      // what fits into the 4 KB of kernel arguments
+#define SLOT_N(x) ((x) & ((1ll << 48) - 1))
+#define GRAD_BF16(x) (((x) >> 61) & 1)
+struct Packed {
+    int start[PACK];
+    Slot slot[PACK];
+    float bias[PACK][2];             // {lr / (1-b1^t), 1 / sqrt(1-b2^t)} of each tensor
+    int count;
+};
+struct Tabled {
+    const Slot* slot;
+    const int* owner;
+};
+__device__ __forceinline__ int slot_of(KARG(Packed)& l, int b) {
     const int lane = threadIdx.x & 63;
-    const bool before = lane < count && starts[lane] <= b;
-    return __popcll(__ballot(before)) - 1;
+    const bool before = lane < l.count && l.start[lane] <= b;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
 }
+__device__ __forceinline__ int slot_of(KARG(Tabled)& l, int b) { return ((KARG(int)*)l.owner)[b]; }
+__device__ __forceinline__ KARG(Slot)& slot_at(KARG(Packed)& l, int i) { return l.slot[i]; }
+__device__ __forceinline__ KARG(Slot)& slot_at(KARG(Tabled)& l, int i) { return ((KARG(Slot)*)l.slot)[i]; }
 
 // ---- the norm -----------------------------------------------------------------------------------------------------
 // Sums of squares are kept in 64 bits from the first element on: fp32 squares overflow from |g| = 1.8e19 on, and long
 // fp32 sums lose the small gradients.  The fp64 FMA runs at the fp32 rate on this chip, so the pass stays a read.
-struct NormSlot { void* g; int64_t n; };          // n: bits 0..47 elements, bit 60: bf16
-struct NormArgs {
-    int start[OPT_SLOTS];
-    NormSlot slot[OPT_SLOTS];
-    double* part;
-    int count, chunks;
-};
-#define OPT_N(x) ((x) & ((1ll << 48) - 1))
-#define NORM_CHUNK 4096
-
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
@@ -94,33 +114,55 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 }
 
 template <typename T>
-__device__ __forceinline__ double chunk_sumsq(const T* g, int64_t left) {
-    double s[4] = {0., 0., 0., 0.};
+__device__ __forceinline__ void add_squares(const float x[4], double s[4]) {
 #pragma unroll
-    for (int u = 0; u < NORM_CHUNK / (4 * OPT_THREADS); ++u) {
-        const int64_t i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
-        if (i < left) {
-            float x[4];
-            load4(g + i, left - i < 4 ? (int)(left - i) : 4, x);
+    for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
+}
+// n consecutive elements by the block; NORM_U loads of a thread in flight
+#define NORM_U 8
+template <typename T>
+__device__ __forceinline__ void run_sumsq(const T* g, int64_t n, double s[4]) {
+    const int64_t step = 4 * OPT_THREADS;
+    int64_t i = 4 * (int)threadIdx.x;
+    for (; i + (NORM_U - 1) * step + 4 <= n; i += NORM_U * step) {
+        float x[NORM_U][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
-        }
+        for (int u = 0; u < NORM_U; ++u) Quad<T>::load(g + i + u * step, x[u]);
+#pragma unroll
+        for (int u = 0; u < NORM_U; ++u) add_squares<T>(x[u], s);
     }
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    for (; i < n; i += step) {
+        float x[4];
+        load4(g + i, n - i < 4 ? (int)(n - i) : 4, x);
+        add_squares<T>(x, s);
+    }
 }
 
-__global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs by_value) {
-    KARG(NormArgs)& a = *kernel_args<NormArgs>();
+template <typename L> struct NormArgs {
+    L list;
+    double* part;
+    int chunks;
+};
+template <typename L>
+__global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs<L> by_value) {
+    KARG(NormArgs<L>)& a = *kernel_args<NormArgs<L>>();
     __shared__ double red[4];
-    double s = 0.;
-    for (int b = blockIdx.x; b < a.chunks; b += gridDim.x) {
-        const int i = __builtin_amdgcn_readfirstlane(find_slot(a.start, a.count, b));
-        const int64_t n = a.slot[i].n, first = (int64_t)(b - a.start[i]) * NORM_CHUNK, left = OPT_N(n) - first;
-        s += ((n >> 60) & 1) ? chunk_sumsq((const unsigned short*)a.slot[i].g + first, left)
-                       : chunk_sumsq((const float*)a.slot[i].g + first, left);
+    double s[4] = {0., 0., 0., 0.};
+    // a contiguous share of the chunks for each block, walked tensor by tensor
+    int b = (int)((int64_t)a.chunks * blockIdx.x / gridDim.x);
+    const int end = (int)((int64_t)a.chunks * (blockIdx.x + 1) / gridDim.x);
+    while (b < end) {
+        KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
+        const int64_t flags = t.n, first = (int64_t)(b - t.start) * OPT_CHUNK;
+        int64_t n = SLOT_N(flags) - first;
+        const int64_t most = (int64_t)(end - b) * OPT_CHUNK;
+        if (n > most) n = most;
+        if (GRAD_BF16(flags)) run_sumsq((const unsigned short*)t.g + first, n, s);
+        else run_sumsq((const float*)t.g + first, n, s);
+        b += (int)((n + OPT_CHUNK - 1) / OPT_CHUNK);
     }
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = s;
+    const double sum = block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
 }
 
 struct ClipArgs { const double* part; double max_norm; float* norm; float* coef; int parts; };     // norm, coef: written where not NULL
@@ -136,43 +178,51 @@ __device__ __forceinline__ float clip_coef(const ClipArgs& c, double* red, bool 
     if (write_norm && threadIdx.x == 0 && c.coef) *c.coef = coef;
     return coef;
 }
+__device__ __forceinline__ ClipArgs clip_args(KARG(ClipArgs)& c) { return {c.part, c.max_norm, c.norm, c.coef, c.parts}; }
 
 __global__ __launch_bounds__(OPT_THREADS) void norm_finish_kernel(ClipArgs c) {
     __shared__ double red[4];
     (void)clip_coef(c, red, true);
 }
 
-#define SCALE_CHUNK 4096
-struct ScaleArgs {
-    int start[OPT_SLOTS];
-    NormSlot slot[OPT_SLOTS];
+template <typename L> struct ScaleArgs {
+    L list;
     ClipArgs clip;
-    int count, first_launch;
+    int first_launch;
 };
 template <typename T>
 __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
+    float x[OPT_U][4];
+    if (left >= OPT_CHUNK) {
 #pragma unroll
-    for (int u = 0; u < SCALE_CHUNK / (4 * OPT_THREADS); ++u) {
-        const int64_t i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
-        if (i < left) {
-            const int k = left - i < 4 ? (int)(left - i) : 4;
-            float x[4];
-            load4(g + i, k, x);
+        for (int u = 0; u < OPT_U; ++u) Quad<T>::load(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= c;
-            store4(g + i, k, x);
+        for (int u = 0; u < OPT_U; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] *= c;
+            Quad<T>::store(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
         }
+        return;
+    }
+    for (int i = 4 * (int)threadIdx.x; i < left; i += 4 * OPT_THREADS) {
+        const int k = left - i < 4 ? (int)(left - i) : 4;
+        load4(g + i, k, x[0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[0][e] *= c;
+        store4(g + i, k, x[0]);
     }
 }
-__global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs by_value) {
-    KARG(ScaleArgs)& a = *kernel_args<ScaleArgs>();
+template <typename L>
+__global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by_value) {
+    KARG(ScaleArgs<L>)& a = *kernel_args<ScaleArgs<L>>();
     __shared__ double red[4];
-    const float c = clip_coef({a.clip.part, a.clip.max_norm, a.clip.norm, nullptr, a.clip.parts}, red, a.first_launch && blockIdx.x == 0);
+    const float c = clip_coef(clip_args(a.clip), red, a.first_launch && blockIdx.x == 0);
     if (c == 1.f) return;                               // x * 1 = x for every x
-    const int b = blockIdx.x, i = __builtin_amdgcn_readfirstlane(find_slot(a.start, a.count, b));
-    const int64_t n = a.slot[i].n, first = (int64_t)(b - a.start[i]) * SCALE_CHUNK, left = OPT_N(n) - first;
-    if ((n >> 60) & 1) chunk_scale((unsigned short*)a.slot[i].g + first, left, c);
-    else chunk_scale((float*)a.slot[i].g + first, left, c);
+    const int b = blockIdx.x;
+    KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
+    const int64_t flags = t.n, first = (int64_t)(b - t.start) * OPT_CHUNK, left = SLOT_N(flags) - first;
+    if (GRAD_BF16(flags)) chunk_scale((unsigned short*)t.g + first, left, c);
+    else chunk_scale((float*)t.g + first, left, c);
 }
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------
@@ -180,25 +230,18 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs by_va
 //   p  <- (1 - lr wd) p - lr / (1-b1^t) * m / (sqrt(v) / sqrt(1-b2^t) + eps)
 // Every operation is rounded by itself (no contraction, IEEE division and square root), so the step is the same fp32
 // arithmetic as the formula written with elementary tensor operations, bit for bit.
-struct AdamSlot {
-    void* p; const void* g; void* m; void* v; float* ms; float* vs;
-    int64_t n;                       // bits 0..47 elements, bit 60: bf16 parameter, bit 61: bf16 gradient
-    float step_size, inv_bc2;        // lr / (1-b1^t), 1 / sqrt(1-b2^t)
-    int index;                       // of the tensor in the caller's list (its place in the clock)
-};
-#define ADAM_SLOTS 52                // what fits into the 4 KB of kernel arguments
-struct AdamArgs {
-    int start[ADAM_SLOTS];
-    AdamSlot slot[ADAM_SLOTS];
+struct AdamC { float decay, b1, c1, b2, c2, eps, step_size, inv_bc2, coef; };
+template <typename L> struct AdamArgs {
+    L list;
     ClipArgs clip;                   // clip.part NULL: no clipping
     const float* coef;               // coefficient that an earlier norm left; or NULL
     const float* clock;              // device-side step counters: decay, then {step_size, inv_bc2} per tensor; or NULL
-    float decay, b1, c1, b2, c2, eps;
-    int count, first_launch;
+    float decay, b1, c1, b2, c2, eps, step_size, inv_bc2;
+    int first_launch;
 };
-static_assert(sizeof(AdamArgs) <= 4096 && sizeof(ScaleArgs) <= 4096 && sizeof(NormArgs) <= 4096, "kernel arguments");
-
-struct AdamC { float decay, b1, c1, b2, c2, eps, step_size, inv_bc2, coef; };
+static_assert(sizeof(AdamArgs<Packed>) <= 4096 && sizeof(ScaleArgs<Packed>) <= 4096 && sizeof(NormArgs<Packed>) <= 4096, "kernel arguments");
+__device__ __forceinline__ void own_bias(KARG(Packed)& l, int i, AdamC& c) { c.step_size = l.bias[i][0]; c.inv_bc2 = l.bias[i][1]; }
+__device__ __forceinline__ void own_bias(KARG(Tabled)&, int, AdamC&) {}     // one step number for the whole list
 
 __device__ __forceinline__ void adam_moments(float g, float& m, float& v, const AdamC& c) {
     g = g * c.coef;
@@ -209,24 +252,47 @@ __device__ __forceinline__ float adam_update(float p, float m, float r, const Ad
     const float denom = r * c.inv_bc2 + c.eps;
     return p * c.decay - (m / denom) * c.step_size;
 }
-
-template <typename PT, typename GT>
-__device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float* v, int64_t left, int elems, const AdamC& c) {
-    for (int i = 4 * (int)threadIdx.x; i < elems && i < left; i += 4 * OPT_THREADS) {
-        const int k = left - i < 4 ? (int)(left - i) : 4;
-        float xp[4], xg[4], xm[4], xv[4];
-        load4(p + i, k, xp);
-        load4(g + i, k, xg);
-        load4(m + i, k, xm);
-        load4(v + i, k, xv);
+__device__ __forceinline__ void adam32_quad(float p[4], const float g[4], float m[4], float v[4], const AdamC& c) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            adam_moments(xg[e], xm[e], xv[e], c);
-            xp[e] = adam_update(xp[e], xm[e], sqrtf(xv[e]), c);
+    for (int e = 0; e < 4; ++e) {
+        adam_moments(g[e], m[e], v[e], c);
+        p[e] = adam_update(p[e], m[e], sqrtf(v[e]), c);
+    }
+}
+
+// a chunk: every load of a thread is requested before the first is used
+template <typename PT, typename GT>
+__device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float* v, int64_t left, const AdamC& c) {
+    float xp[OPT_U][4], xg[OPT_U][4], xm[OPT_U][4], xv[OPT_U][4];
+    if (left >= OPT_CHUNK) {
+#pragma unroll
+        for (int u = 0; u < OPT_U; ++u) {
+            const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
+            Quad<PT>::load(p + i, xp[u]);
+            Quad<GT>::load(g + i, xg[u]);
+            Quad<float>::load(m + i, xm[u]);
+            Quad<float>::load(v + i, xv[u]);
         }
-        store4(m + i, k, xm);
-        store4(v + i, k, xv);
-        store4(p + i, k, xp);
+#pragma unroll
+        for (int u = 0; u < OPT_U; ++u) {
+            const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
+            adam32_quad(xp[u], xg[u], xm[u], xv[u], c);
+            Quad<float>::store(m + i, xm[u]);
+            Quad<float>::store(v + i, xv[u]);
+            Quad<PT>::store(p + i, xp[u]);
+        }
+        return;
+    }
+    for (int i = 4 * (int)threadIdx.x; i < left; i += 4 * OPT_THREADS) {
+        const int k = left - i < 4 ? (int)(left - i) : 4;
+        load4(p + i, k, xp[0]);
+        load4(g + i, k, xg[0]);
+        load4(m + i, k, xm[0]);
+        load4(v + i, k, xv[0]);
+        adam32_quad(xp[0], xg[0], xm[0], xv[0], c);
+        store4(m + i, k, xm[0]);
+        store4(v + i, k, xv[0]);
+        store4(p + i, k, xp[0]);
     }
 }
 
@@ -237,9 +303,10 @@ __device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float
 //  - sqrt(v) > 0 never gets code 0: rounding a denominator down to eps would blow its entry's update up.
 //  - the update of p uses the moments of this step before they are rounded.
 //  - an entry that is not finite takes the NaN code and is left out of absmax: its neighbours keep their values.
+#define FLOAT_MAX 3.4028234663852886e38f
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
-    return a <= 3.4028234663852886e38f ? a : 0.f;
+    return a <= FLOAT_MAX ? a : 0.f;
 }
 __device__ __forceinline__ float quant_scale(float amax) {
     const float s = amax * (1.f / E4M3_MAX);
@@ -266,77 +333,127 @@ __device__ __forceinline__ void store_codes(unsigned char* p, int k, unsigned w)
     for (int e = 0; e < 3; ++e) if (e < k) p[e] = (unsigned char)(w >> (8 * e));
 }
 
-// one QBLOCK per wave: `left` elements from its first on
-template <typename PT, typename GT>
-__device__ __forceinline__ void adam8_block(PT* p, const GT* g, unsigned char* m, unsigned char* r, float* ms, float* rs,
-                                            int64_t left, const AdamC& c) {
-    const int i = 4 * (threadIdx.x & 63);
-    const int k = left - i >= 4 ? 4 : left > i ? (int)(left - i) : 0;
-    float xp[4] = {0.f, 0.f, 0.f, 0.f}, xg[4] = {0.f, 0.f, 0.f, 0.f}, xm[4] = {0.f, 0.f, 0.f, 0.f}, xr[4] = {0.f, 0.f, 0.f, 0.f};
-    if (k) {
-        load4(p + i, k, xp);
-        load4(g + i, k, xg);
-        from_e4m3x4(load_codes(m + i, k), *ms, xm);
-        from_e4m3x4(load_codes(r + i, k), *rs, xr);
-    }
+// maximum over the wave's lanes, in every lane
+__device__ __forceinline__ float wave_max_all(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));      // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp_f32<0x4E>(v));      // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp_f32<0x141>(v));     // row_half_mirror
+    v = fmaxf(v, dpp_f32<0x140>(v));     // row_mirror
+    const float r0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0));
+    const float r1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16));
+    const float r2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32));
+    const float r3 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48));
+    return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+}
+
+// four elements of each lane, one QBLOCK of the wave: new moments, the update of p, the codes; -> the two scales
+__device__ __forceinline__ void adam8_quad(float p[4], const float g[4], unsigned& mw, unsigned& rw, float& ms, float& rs, const AdamC& c) {
+    float m[4], r[4];
+    from_e4m3x4(mw, ms, m);
+    from_e4m3x4(rw, rs, r);
     float am = 0.f, ar = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float v = xr[e] * xr[e];
-        adam_moments(xg[e], xm[e], v, c);
-        xr[e] = sqrtf(v);
-        xp[e] = adam_update(xp[e], xm[e], xr[e], c);
-        am = fmaxf(am, finite_abs(xm[e]));
-        ar = fmaxf(ar, finite_abs(xr[e]));
+        float v = r[e] * r[e];
+        adam_moments(g[e], m[e], v, c);
+        r[e] = sqrtf(v);
+        p[e] = adam_update(p[e], m[e], r[e], c);
+        am = fmaxf(am, finite_abs(m[e]));
+        ar = fmaxf(ar, finite_abs(r[e]));
     }
-    const float sm = quant_scale(wave_max(am)), sr = quant_scale(wave_max(ar));
-    const float im = 1.f / sm, ir = 1.f / sr;
+    ms = quant_scale(wave_max_all(am));
+    rs = quant_scale(wave_max_all(ar));
+    const float im = 1.f / ms, ir = 1.f / rs;
     float ym[4], yr[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        ym[e] = fabsf(xm[e]) <= 3.4028234663852886e38f ? xm[e] * im : __builtin_nanf("");
-        yr[e] = xr[e] <= 3.4028234663852886e38f ? xr[e] * ir : __builtin_nanf("");
+        ym[e] = fabsf(m[e]) <= FLOAT_MAX ? m[e] * im : __builtin_nanf("");
+        yr[e] = r[e] <= FLOAT_MAX ? r[e] * ir : __builtin_nanf("");
         if (yr[e] > 0.f && yr[e] < 0.001953125f) yr[e] = 0.001953125f;       // 2^-9, the smallest code
     }
-    if (k) {
-        store_codes(m + i, k, e4m3x4(ym));
-        store_codes(r + i, k, e4m3x4(yr));
-        store4(p + i, k, xp);
-    }
-    if ((threadIdx.x & 63) == 0) { *ms = sm; *rs = sr; }
+    mw = e4m3x4(ym);
+    rw = e4m3x4(yr);
 }
 
-#define ADAM_CHUNK 4096
-template <int BITS, typename PT, typename GT>
-__device__ __forceinline__ void adam_chunk(const AdamSlot& s, int64_t first, int64_t left, const AdamC& c) {
-    if constexpr (BITS == 32) {
-        adam32_chunk((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, ADAM_CHUNK, c);
-    } else {
-        for (int b = threadIdx.x >> 6; b < ADAM_CHUNK / QBLOCK && (int64_t)b * QBLOCK < left; b += OPT_THREADS / 64) {
-            const int64_t at = first + b * QBLOCK, q = at / QBLOCK;
-            adam8_block((PT*)s.p + at, (const GT*)s.g + at, (unsigned char*)s.m + at, (unsigned char*)s.v + at, s.ms + q, s.vs + q,
-                        left - b * QBLOCK, c);
+// wave w of the block: blocks w, w + 4, ... of the chunk
+template <typename PT, typename GT>
+__device__ __forceinline__ void adam8_chunk(PT* p, const GT* g, unsigned char* m, unsigned char* r, float* ms, float* rs, int64_t left,
+                                            const AdamC& c) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    float xp[OPT_U][4], xg[OPT_U][4], sm[OPT_U], sr[OPT_U];
+    unsigned cm[OPT_U], cr[OPT_U];
+    if (left >= OPT_CHUNK) {
+#pragma unroll
+        for (int u = 0; u < OPT_U; ++u) {
+            const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
+            sm[u] = ms[q];
+            sr[u] = rs[q];
+            cm[u] = *reinterpret_cast<const unsigned*>(m + i);
+            cr[u] = *reinterpret_cast<const unsigned*>(r + i);
+            Quad<GT>::load(g + i, xg[u]);
+            Quad<PT>::load(p + i, xp[u]);
         }
+#pragma unroll
+        for (int u = 0; u < OPT_U; ++u) {
+            const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
+            adam8_quad(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c);
+            *reinterpret_cast<unsigned*>(m + i) = cm[u];
+            *reinterpret_cast<unsigned*>(r + i) = cr[u];
+            Quad<PT>::store(p + i, xp[u]);
+            if (lane == 0) { ms[q] = sm[u]; rs[q] = sr[u]; }
+        }
+        return;
+    }
+    for (int q = w; q * QBLOCK < left; q += OPT_THREADS / 64) {
+        const int i = q * QBLOCK + 4 * lane;
+        const int k = left - i >= 4 ? 4 : left > i ? (int)(left - i) : 0;
+        sm[0] = ms[q];
+        sr[0] = rs[q];
+        cm[0] = cr[0] = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) xp[0][e] = xg[0][e] = 0.f;
+        if (k) {
+            load4(p + i, k, xp[0]);
+            load4(g + i, k, xg[0]);
+            cm[0] = load_codes(m + i, k);
+            cr[0] = load_codes(r + i, k);
+        }
+        adam8_quad(xp[0], xg[0], cm[0], cr[0], sm[0], sr[0], c);
+        if (k) {
+            store_codes(m + i, k, cm[0]);
+            store_codes(r + i, k, cr[0]);
+            store4(p + i, k, xp[0]);
+        }
+        if (lane == 0) { ms[q] = sm[0]; rs[q] = sr[0]; }
     }
 }
 
-template <int BITS>
-__global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs by_value) {
-    KARG(AdamArgs)& a = *kernel_args<AdamArgs>();
+template <int BITS, typename PT, typename GT>
+__device__ __forceinline__ void adam_chunk(KARG(Slot)& s, int64_t first, int64_t left, const AdamC& c) {
+    if constexpr (BITS == 32)
+        adam32_chunk((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, c);
+    else
+        adam8_chunk((PT*)s.p + first, (const GT*)s.g + first, (unsigned char*)s.m + first, (unsigned char*)s.v + first, s.ms + first / QBLOCK,
+                    s.vs + first / QBLOCK, left, c);
+}
+
+template <int BITS, typename L>
+__global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value) {
+    KARG(AdamArgs<L>)& a = *kernel_args<AdamArgs<L>>();
     __shared__ double red[4];
-    const int b = blockIdx.x, i = __builtin_amdgcn_readfirstlane(find_slot(a.start, a.count, b));
-    KARG(AdamSlot)& k = a.slot[i];
-    const AdamSlot s = {k.p, k.g, k.m, k.v, k.ms, k.vs, k.n, k.step_size, k.inv_bc2, k.index};
-    const int64_t first = (int64_t)(b - a.start[i]) * ADAM_CHUNK, left = OPT_N(s.n) - first;
-    AdamC c = {a.decay, a.b1, a.c1, a.b2, a.c2, a.eps, s.step_size, s.inv_bc2, 1.f};
+    const int b = blockIdx.x, i = slot_of(a.list, b);
+    KARG(Slot)& s = slot_at(a.list, i);
+    const int64_t flags = s.n, first = (int64_t)(b - s.start) * OPT_CHUNK, left = SLOT_N(flags) - first;
+    AdamC c = {a.decay, a.b1, a.c1, a.b2, a.c2, a.eps, a.step_size, a.inv_bc2, 1.f};
+    own_bias(a.list, i, c);
     if (a.clock) {
         c.decay = a.clock[0];
         c.step_size = a.clock[1 + 2 * s.index];
         c.inv_bc2 = a.clock[2 + 2 * s.index];
     }
     if (a.coef) c.coef = *a.coef;
-    if (a.clip.part) c.coef = clip_coef({a.clip.part, a.clip.max_norm, a.clip.norm, nullptr, a.clip.parts}, red, a.first_launch && b == 0);
-    switch ((int)(s.n >> 60) & 3) {
+    if (a.clip.part) c.coef = clip_coef(clip_args(a.clip), red, a.first_launch && b == 0);
+    switch ((int)(flags >> 60) & 3) {
         case 0: adam_chunk<BITS, float, float>(s, first, left, c); break;
         case 1: adam_chunk<BITS, unsigned short, float>(s, first, left, c); break;
         case 2: adam_chunk<BITS, float, unsigned short>(s, first, left, c); break;
@@ -365,109 +482,189 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_clock_kernel(ClockArgs by_v
     a.clock[2 + 2 * (a.base + i)] = (float)(1. / sqrt(1. - pow(a.b2, (double)t)));
 }
 
+// ---- the table of a Tabled list: slots, then the owner of every chunk -----------------------------------------------
+struct TableArgs { Packed list; Slot* slot; int* owner; int chunks, base; };
+static_assert(sizeof(TableArgs) <= 4096, "kernel arguments");
+__global__ __launch_bounds__(OPT_THREADS) void opt_table_kernel(TableArgs by_value) {
+    KARG(TableArgs)& a = *kernel_args<TableArgs>();
+    // block i: tensor i of the launch (its chunks are [start, next tensor's start) of the whole list)
+    const int i = blockIdx.x;
+    KARG(Slot)& s = a.list.slot[i];
+    if (threadIdx.x == 0) a.slot[a.base + i] = Slot{s.p, s.g, s.m, s.v, s.ms, s.vs, s.n, s.start, s.index};
+    const int64_t chunks = (SLOT_N(s.n) + OPT_CHUNK - 1) / OPT_CHUNK;
+    for (int64_t k = threadIdx.x; k < chunks; k += OPT_THREADS) a.owner[s.start + k] = a.base + i;
+}
+
 // ---- host side --------------------------------------------------------------------------------------------------------
-static int64_t chunks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
+static int64_t chunks_of(int64_t n) { return (n + OPT_CHUNK - 1) / OPT_CHUNK; }
 
 static bool bad_grad(const denet_opt_tensor_t& t) {
     return t.n < 0 || t.n >= (1ll << 48) || (t.n > 0 && !t.grad) || (t.grad_dtype != DENET_F32 && t.grad_dtype != DENET_BF16) ||
            ((uintptr_t)t.grad & (t.grad_dtype == DENET_F32 ? 3 : 1));
 }
-static int check_grads(const denet_opt_tensor_t* t, int64_t count) {
+// checks what every call reads; -> the list's chunks and its tensors that have any
+static int check_list(const denet_opt_tensor_t* t, int64_t count, int64_t* chunks_out, int64_t* live_out) {
     if (count < 0 || count > (1ll << 24) || (count > 0 && !t)) return DENET_E_BADARG;
-    int64_t chunks = 0;
+    int64_t chunks = 0, live = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (bad_grad(t[i])) return DENET_E_BADARG;
-        chunks += chunks_of(t[i].n, NORM_CHUNK);
+        chunks += chunks_of(t[i].n);
+        live += t[i].n > 0;
         if (chunks >= (1ll << 31)) return DENET_E_UNSUPPORTED;
+    }
+    *chunks_out = chunks;
+    *live_out = live;
+    return DENET_OK;
+}
+static Slot slot_from(const denet_opt_tensor_t& t, int start, int64_t index) {
+    return {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.avg_scale, t.sq_scale,
+            t.n | ((int64_t)(t.param_dtype == DENET_BF16) << 60) | ((int64_t)(t.grad_dtype == DENET_BF16) << 61), start, (int)index};
+}
+
+static Tabled tabled(const void* table, int64_t live) { return {(const Slot*)table, (const int*)((const Slot*)table + live)}; }
+
+// Runs `launch(list, chunks)` over the list: once with its table, or for every PACK tensors.  `bias(i, out)` fills a packed tensor's constants.
+template <typename Args, typename Bias, typename Launch>
+static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias bias, Launch launch) {
+    int64_t chunks = 0;
+    Packed& l = a.list;
+    l.count = 0;
+    for (int64_t i = 0; i <= count; ++i) {
+        if (l.count == PACK || (i == count && l.count)) {
+            const int rc = launch((int)chunks);
+            if (rc != DENET_OK) return rc;
+            chunks = l.count = 0;
+        }
+        if (i == count || t[i].n == 0) continue;
+        l.start[l.count] = (int)chunks;
+        l.slot[l.count] = slot_from(t[i], (int)chunks, i);
+        bias(t[i], l.bias[l.count]);
+        chunks += chunks_of(t[i].n);
+        ++l.count;
     }
     return DENET_OK;
 }
+static void no_bias(const denet_opt_tensor_t&, float out[2]) { out[0] = out[1] = 0.f; }
 
-// Partial sums of the whole list: at most NORM_PARTS over all launches, shared out by their chunks; -> how many were written.
-static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, double* part, hipStream_t st, int* parts_out) {
-    int64_t total = 0;
-    for (int64_t i = 0; i < count; ++i) total += chunks_of(t[i].n, NORM_CHUNK);
+// Partial sums of the whole list: at most NORM_PARTS, shared out over the launches by their chunks (rounded up); -> how many were written.
+static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, int64_t total, int64_t live, const void* table, double* part,
+                        hipStream_t st, int* parts_out) {
     int parts = 0;
-    NormArgs a;
-    a.count = a.chunks = 0;
-    for (int64_t i = 0; i <= count; ++i) {
-        if (a.count == OPT_SLOTS || (i == count && a.count)) {
-            // (the share is rounded up, so every launch has a block; the list has at most NORM_PARTS / 2 launches, see the workspace)
-            int64_t grid = a.chunks;
-            if (total > NORM_PARTS) grid = (int64_t)a.chunks * (NORM_PARTS - 1) / total + 1;
+    auto grid_of = [&](int64_t chunks) {
+        const int64_t most = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (NORM_PARTS - 1) / total + 1;
+        return most < share ? most : share;
+    };
+    *parts_out = 0;
+    if (!live) return DENET_OK;
+    if (table) {
+        NormArgs<Tabled> a;
+        a.list = tabled(table, live);
+        a.part = part;
+        a.chunks = (int)total;
+        parts = (int)grid_of(total);
+        hipLaunchKernelGGL(grad_sumsq_kernel<Tabled>, dim3((unsigned)parts), dim3(OPT_THREADS), 0, st, a);
+        DENET_CHECK_LAUNCH();
+    } else {
+        NormArgs<Packed> a;
+        const int rc = over_packs(t, count, a, no_bias, [&](int chunks) {
+            const int64_t grid = grid_of(chunks);
             a.part = part + parts;
-            hipLaunchKernelGGL(grad_sumsq_kernel, dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+            a.chunks = chunks;
+            hipLaunchKernelGGL(grad_sumsq_kernel<Packed>, dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
             DENET_CHECK_LAUNCH();
             parts += (int)grid;
-            a.count = a.chunks = 0;
-        }
-        if (i == count || t[i].n == 0) continue;
-        a.start[a.count] = a.chunks;
-        a.slot[a.count] = {t[i].grad, t[i].n | ((int64_t)(t[i].grad_dtype == DENET_BF16) << 60)};
-        a.chunks += (int)chunks_of(t[i].n, NORM_CHUNK);
-        ++a.count;
+            return DENET_OK;
+        });
+        if (rc != DENET_OK) return rc;
     }
     *parts_out = parts;
     return DENET_OK;
 }
 
-// partial sums: NORM_PARTS, one more for each launch (their shares are rounded up); then the clock of a device-side step counter
-static int64_t part_bytes(int64_t count) { return (NORM_PARTS + count / OPT_SLOTS + 1) * (int64_t)sizeof(double); }
+// workspace: NORM_PARTS partial sums, one more for each launch (their shares are rounded up); then the clock of device-side counters
+static int64_t part_bytes(int64_t count) { return (NORM_PARTS + count / PACK + 1) * (int64_t)sizeof(double); }
 
 extern "C" int64_t denet_opt_workspace(int64_t count) {
     if (count < 0 || count > (1ll << 24)) return DENET_E_BADARG;
     return part_bytes(count) + (2 * count + 2) * (int64_t)sizeof(float);
 }
-
 static int check_ws(const void* ws, int64_t ws_bytes, int64_t count) {
     if (!ws || ((uintptr_t)ws & 7)) return DENET_E_BADARG;
     return ws_bytes < denet_opt_workspace(count) ? DENET_E_WORKSPACE : DENET_OK;
 }
 
-extern "C" int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm, float* coef, void* ws,
-                               int64_t ws_bytes, void* stream) {
-    int rc = check_grads(tensors, count);
-    if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
+extern "C" int64_t denet_opt_table_bytes(const denet_opt_tensor_t* tensors, int64_t count) {
+    int64_t chunks, live;
+    const int rc = check_list(tensors, count, &chunks, &live);
+    return rc != DENET_OK ? rc : live * (int64_t)sizeof(Slot) + chunks * (int64_t)sizeof(int);
+}
+extern "C" int denet_opt_table(const denet_opt_tensor_t* tensors, int64_t count, void* table, int64_t table_bytes, void* stream) {
+    int64_t chunks, live, base = 0, done = 0;
+    int rc = check_list(tensors, count, &chunks, &live);
     if (rc != DENET_OK) return rc;
-    if (!norm || (coef && !(max_norm >= 0.))) return DENET_E_BADARG;
-    int parts = 0;
-    rc = launch_sumsq(tensors, count, (double*)ws, (hipStream_t)stream, &parts);
-    if (rc != DENET_OK) return rc;
-    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(OPT_THREADS), 0, (hipStream_t)stream,
-                       ClipArgs{(const double*)ws, max_norm, norm, coef, parts});
+    if (!table || ((uintptr_t)table & 15)) return DENET_E_BADARG;
+    if (table_bytes < denet_opt_table_bytes(tensors, count)) return DENET_E_WORKSPACE;
+    TableArgs a;
+    a.slot = (Slot*)table;
+    a.owner = (int*)(a.slot + live);
+    return over_packs(tensors, count, a, no_bias, [&](int n) {
+        for (int i = 0; i < a.list.count; ++i) a.list.slot[i].start += (int)done;
+        a.chunks = n;
+        a.base = (int)base;
+        hipLaunchKernelGGL(opt_table_kernel, dim3((unsigned)a.list.count), dim3(OPT_THREADS), 0, (hipStream_t)stream, a);
+        DENET_CHECK_LAUNCH();
+        base += a.list.count;
+        done += n;
+        return DENET_OK;
+    });
+}
+
+static bool bad_table(const void* table) { return (uintptr_t)table & 15; }
+
+static int finish_norm(const ClipArgs& c, hipStream_t st) {
+    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(OPT_THREADS), 0, st, c);
     DENET_CHECK_LAUNCH();
     return DENET_OK;
 }
 
-extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm, void* ws,
-                               int64_t ws_bytes, void* stream) {
-    int rc = check_grads(tensors, count);
+extern "C" int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, float* coef,
+                               void* ws, int64_t ws_bytes, void* stream) {
+    int64_t chunks, live;
+    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
-    if (!norm || !(max_norm >= 0.)) return DENET_E_BADARG;
-    hipStream_t st = (hipStream_t)stream;
-    int parts = 0;
-    rc = launch_sumsq(tensors, count, (double*)ws, st, &parts);
+    if (!norm || bad_table(table) || (coef && !(max_norm >= 0.))) return DENET_E_BADARG;
+    rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, (hipStream_t)stream, &parts);
+    return rc != DENET_OK ? rc : finish_norm({(const double*)ws, max_norm, norm, coef, parts}, (hipStream_t)stream);
+}
+
+extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, void* ws,
+                               int64_t ws_bytes, void* stream) {
+    int64_t chunks, live;
+    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
+    if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
-    if (!parts) return denet_grad_norm(tensors, count, max_norm, norm, nullptr, ws, ws_bytes, stream);      // nothing but empty tensors: norm 0
-    ScaleArgs a;
-    a.clip = {(const double*)ws, max_norm, norm, nullptr, parts};
-    a.count = 0;
-    a.first_launch = 1;
-    int chunks = 0;
-    for (int64_t i = 0; i <= count; ++i) {
-        if (a.count == OPT_SLOTS || (i == count && a.count)) {
-            hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
-            DENET_CHECK_LAUNCH();
-            a.first_launch = a.count = chunks = 0;
-        }
-        if (i == count || tensors[i].n == 0) continue;
-        a.start[a.count] = chunks;
-        a.slot[a.count] = {tensors[i].grad, tensors[i].n | ((int64_t)(tensors[i].grad_dtype == DENET_BF16) << 60)};
-        chunks += (int)chunks_of(tensors[i].n, SCALE_CHUNK);
-        ++a.count;
+    if (!norm || bad_table(table) || !(max_norm >= 0.)) return DENET_E_BADARG;
+    hipStream_t st = (hipStream_t)stream;
+    rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, st, &parts);
+    if (rc != DENET_OK) return rc;
+    const ClipArgs clip = {(const double*)ws, max_norm, norm, nullptr, parts};
+    if (!live) return finish_norm(clip, st);                                   // nothing but empty tensors: norm 0
+    if (table) {
+        const ScaleArgs<Tabled> a = {tabled(table, live), clip, 1};
+        hipLaunchKernelGGL(grad_scale_kernel<Tabled>, dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
+        DENET_CHECK_LAUNCH();
+        return DENET_OK;
     }
-    return DENET_OK;
+    ScaleArgs<Packed> a;
+    a.clip = clip;
+    a.first_launch = 1;
+    return over_packs(tensors, count, a, no_bias, [&](int n) {
+        hipLaunchKernelGGL(grad_scale_kernel<Packed>, dim3((unsigned)n), dim3(OPT_THREADS), 0, st, a);
+        DENET_CHECK_LAUNCH();
+        a.first_launch = 0;
+        return DENET_OK;
+    });
 }
 
 static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
@@ -479,43 +676,49 @@ static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
     return bits == 8 && (!t.avg_scale || !t.sq_scale || ((uintptr_t)t.avg_scale & 3) || ((uintptr_t)t.sq_scale & 3));
 }
 
-extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, int bits, const denet_adamw_t* h, float* norm,
-                                void* ws, int64_t ws_bytes, void* stream) {
-    if (!h || (bits != 32 && bits != 8)) return DENET_E_BADARG;
+template <typename L>
+static void launch_adamw(int bits, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
+    if (bits == 8) hipLaunchKernelGGL((adamw_kernel<8, L>), dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
+    else hipLaunchKernelGGL((adamw_kernel<32, L>), dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
+}
+
+extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, const void* table, int bits, const denet_adamw_t* h,
+                                float* norm, void* ws, int64_t ws_bytes, void* stream) {
+    if (!h || bad_table(table) || (bits != 32 && bits != 8)) return DENET_E_BADARG;
     if (!(h->lr >= 0.) || !(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.) ||
-        !(h->weight_decay >= 0.)) return DENET_E_BADARG;
-    int rc = check_grads(tensors, count);
+        !(h->weight_decay >= 0.) || h->max_norm != h->max_norm) return DENET_E_BADARG;
+    int64_t chunks, live;
+    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
     if (rc != DENET_OK) return rc;
-    for (int64_t i = 0; i < count; ++i)
+    bool one_step = true;
+    int64_t t_one = 0;
+    for (int64_t i = 0; i < count; ++i) {
         if (bad_tensor(tensors[i], bits, !h->device_steps)) return DENET_E_BADARG;
-    if (h->max_norm != h->max_norm) return DENET_E_BADARG;
+        if (tensors[i].n == 0) continue;
+        if (!t_one) t_one = tensors[i].step;
+        one_step = one_step && tensors[i].step == t_one;
+    }
     const bool clip = h->max_norm >= 0.;
     if (clip || h->device_steps) {
         rc = check_ws(ws, ws_bytes, count);
         if (rc != DENET_OK) return rc;
     }
-    if (clip && !norm) return DENET_E_BADARG;
-    if ((h->lr_dev && !h->device_steps) || (clip && h->coef)) return DENET_E_BADARG;
+    if ((clip && !norm) || (h->lr_dev && !h->device_steps) || (clip && h->coef)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    AdamArgs a;
-    a.clip = {nullptr, 0., nullptr, nullptr, 0};
-    a.coef = h->coef;
+    ClipArgs ca = {nullptr, 0., nullptr, nullptr, 0};
     if (clip) {
-        int parts = 0;
-        rc = launch_sumsq(tensors, count, (double*)ws, st, &parts);
+        rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, st, &parts);
         if (rc != DENET_OK) return rc;
-        if (!parts) {
-            rc = denet_grad_norm(tensors, count, h->max_norm, norm, nullptr, ws, ws_bytes, stream);
-            if (rc != DENET_OK) return rc;
-        }
-        a.clip = {(const double*)ws, h->max_norm, norm, nullptr, parts};
+        ca = {(const double*)ws, h->max_norm, norm, nullptr, parts};
+        if (!live) return finish_norm(ca, st);
     }
-    a.clock = nullptr;
+    if (!live) return DENET_OK;
+    const float* clock = nullptr;
     if (h->device_steps) {
         ClockArgs k;
         k.lr = h->lr; k.wd = h->weight_decay; k.b1 = h->beta1; k.b2 = h->beta2;
         k.lr_dev = h->lr_dev;
-        k.clock = (float*)((char*)ws + part_bytes(count));
+        clock = k.clock = (float*)((char*)ws + part_bytes(count));
         for (int64_t i = 0; i < count; i += CLOCK_SLOTS) {
             k.base = (int)i;
             k.count = (int)(count - i < CLOCK_SLOTS ? count - i : CLOCK_SLOTS);
@@ -523,39 +726,53 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
             hipLaunchKernelGGL(adamw_clock_kernel, dim3(1), dim3(OPT_THREADS), 0, st, k);
             DENET_CHECK_LAUNCH();
         }
-        a.clock = k.clock;
     }
-    a.decay = (float)(1. - h->lr * h->weight_decay);
-    a.b1 = (float)h->beta1;
-    a.c1 = (float)(1. - h->beta1);
-    a.b2 = (float)h->beta2;
-    a.c2 = (float)(1. - h->beta2);
-    a.eps = (float)h->eps;
-    a.count = 0;
-    a.first_launch = 1;
-    int chunks = 0;
     int64_t t_last = 0;
-    float step_size = 0.f, inv_bc2 = 0.f;
-    for (int64_t i = 0; i <= count; ++i) {
-        if (a.count == ADAM_SLOTS || (i == count && a.count)) {
-            if (bits == 8) hipLaunchKernelGGL(adamw_kernel<8>, dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
-            else hipLaunchKernelGGL(adamw_kernel<32>, dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
-            DENET_CHECK_LAUNCH();
-            a.first_launch = a.count = chunks = 0;
-        }
-        if (i == count || tensors[i].n == 0) continue;
-        const denet_opt_tensor_t& t = tensors[i];
+    float bias_last[2] = {0.f, 0.f};
+    auto bias = [&](const denet_opt_tensor_t& t, float out[2]) {
         if (!h->device_steps && t.step != t_last) {
             t_last = t.step;
-            step_size = (float)(h->lr / (1. - pow(h->beta1, (double)t.step)));
-            inv_bc2 = (float)(1. / sqrt(1. - pow(h->beta2, (double)t.step)));
+            bias_last[0] = (float)(h->lr / (1. - pow(h->beta1, (double)t.step)));
+            bias_last[1] = (float)(1. / sqrt(1. - pow(h->beta2, (double)t.step)));
         }
-        a.start[a.count] = chunks;
-        a.slot[a.count] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.avg_scale, t.sq_scale,
-                           t.n | ((int64_t)(t.param_dtype == DENET_BF16) << 60) | ((int64_t)(t.grad_dtype == DENET_BF16) << 61),
-                           step_size, inv_bc2, (int)i};
-        chunks += (int)chunks_of(t.n, ADAM_CHUNK);
-        ++a.count;
+        out[0] = bias_last[0];
+        out[1] = bias_last[1];
+    };
+    auto fill = [&](auto& a) {
+        a.clip = ca;
+        a.coef = h->coef;
+        a.clock = clock;
+        a.decay = (float)(1. - h->lr * h->weight_decay);
+        a.b1 = (float)h->beta1;
+        a.c1 = (float)(1. - h->beta1);
+        a.b2 = (float)h->beta2;
+        a.c2 = (float)(1. - h->beta2);
+        a.eps = (float)h->eps;
+        a.step_size = a.inv_bc2 = 0.f;
+        a.first_launch = 1;
+    };
+    if (table && (one_step || h->device_steps)) {
+        AdamArgs<Tabled> a;
+        fill(a);
+        a.list = tabled(table, live);
+        if (!h->device_steps) {
+            denet_opt_tensor_t t = {};
+            t.step = t_one;
+            float b[2];
+            bias(t, b);
+            a.step_size = b[0];
+            a.inv_bc2 = b[1];
+        }
+        launch_adamw(bits, chunks, a, st);
+        DENET_CHECK_LAUNCH();
+        return DENET_OK;
     }
-    return DENET_OK;
+    AdamArgs<Packed> a;
+    fill(a);
+    return over_packs(tensors, count, a, bias, [&](int n) {
+        launch_adamw(bits, n, a, st);
+        DENET_CHECK_LAUNCH();
+        a.first_launch = 0;
+        return DENET_OK;
+    });
 }

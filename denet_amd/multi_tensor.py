@@ -1,8 +1,9 @@
 """Operators over lists of tensors: the norm of a gradient list, its clipping, and the AdamW step (include/denet_hip.h, section O).
 
-A *plan* checks a list of tensors once and holds the table that the library reads at every call; like a bound step
-(`_lib.bind`) it keeps the tensors alive, and they stay in place (same storage, type and shape) while it is used.
-The functions without a plan check and pack the list at every call.
+A *plan* checks a list of tensors once and holds the table that the library reads at every call, on the host and on the device;
+like a bound step (`_lib.bind`) it keeps the tensors alive, and they stay in place (same storage, type and shape) while it is
+used.  Building one waits for the current stream.  The functions without a plan check the list at every call and hand it over as
+kernel arguments, which takes a launch for every 52 tensors.
 
 Tensors are fp32 or bf16, dense (contiguous in some order of their dimensions, all tensors of one parameter in the same order),
 and of one device.  Calls go to torch's current stream of that device; norms are fresh 0-d fp32 tensors, workspaces come from
@@ -96,7 +97,7 @@ def _first_device(tensors, what):
 class _Table:
     """The host table of denet_opt_tensor_t rows and the calls on it."""
 
-    def __init__(self, rows, count, device, keep):
+    def __init__(self, rows, count, device, keep, once):
         self.buf = array.array("q", rows)
         self.addr = self.buf.buffer_info()[0]
         self.count = count
@@ -104,6 +105,18 @@ class _Table:
         self.index = device.index if device is not None else None
         self.keep = keep
         self.ws_bytes = _lib.query("denet_opt_workspace", count)
+        # device-side copy of the list, for plans that are used again: then every call is one launch.  It is complete
+        # when the constructor returns, so the plan may be used on any stream.  (Not while a graph is being captured.)
+        self.table = None
+        if not once and not torch.cuda.is_current_stream_capturing():
+            nbytes = int(_lib.load().denet_opt_table_bytes(self.addr, count))
+            if nbytes > 0:
+                table = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                self._run("denet_opt_table", table.data_ptr(), nbytes)
+                torch.cuda.current_stream(self.index).synchronize()
+                self.table, self.table_addr = table, table.data_ptr()
+        if self.table is None:
+            self.table_addr = None
 
     def ws(self):
         return torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
@@ -113,6 +126,9 @@ class _Table:
 
     def call(self, name, *args):
         """`args` end before the stream; raw addresses and numbers."""
+        self._run(name, self.table_addr, *args)
+
+    def _run(self, name, *args):
         fn = getattr(_lib.load(), name)
         if self.index != torch.cuda.current_device():
             with torch.cuda.device(self.index):
@@ -133,7 +149,7 @@ def _norm_limit(max_norm):
 class GradNormPlan:
     """The L2 norm over every element of a list of tensors, and clipping by it (torch.nn.utils.clip_grad_norm_)."""
 
-    def __init__(self, grads):
+    def __init__(self, grads, _once=False):
         grads = list(grads)
         device, index = _first_device(grads, "GradNormPlan")
         addresses = _checked(grads, "gradient", _CODE, device, index)
@@ -143,7 +159,7 @@ class GradNormPlan:
         self.grads = grads
         self._versioned = [g for g in grads if not g.is_inference()]
         self._disjoint = False
-        self._table = _Table(rows, len(grads), device, grads)
+        self._table = _Table(rows, len(grads), device, grads, _once)
 
     def norm(self):
         """sqrt(sum of squares), accumulated in 64 bits: a 0-d fp32 tensor."""
@@ -183,7 +199,7 @@ class AdamWPlan:
     steps: device int64 counters, one 0-d (or one-element) tensor per parameter, advanced by every `step()`; then `step` is not passed and
     the call may be captured into a graph."""
 
-    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None, steps=None, _disjoint=False):
+    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None, steps=None, _once=False, _disjoint=False):
         params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
         if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
             raise DenetHipError("AdamWPlan: scales for both states or for none")
@@ -229,7 +245,7 @@ class AdamWPlan:
         rows = [w for row in zip(at[0], at[1], at[2], at[3], scales[0], scales[1], sizes, [1] * n, counters, codes) for w in row]
         self.device_steps = steps is not None
         self._versioned = [t for t in params if not t.is_inference()]
-        self._table = _Table(rows, n, device, lists)
+        self._table = _Table(rows, n, device, lists, _once)
         self._hyper = h = _lib.AdamWHyper()
         h.device_steps = 1 if self.device_steps else 0
         self._hyper_addr = ctypes.addressof(h)
@@ -304,14 +320,14 @@ class AdamWPlan:
 
 def grad_norm(grads):
     """The L2 norm over every element of the tensors: a 0-d fp32 tensor."""
-    return GradNormPlan(grads).norm()
+    return GradNormPlan(grads, _once=True).norm()
 
 
 def clip_grads_(grads, max_norm):
     """Scales the tensors in place so that their common L2 norm is at most max_norm; returns the norm before."""
-    return GradNormPlan(grads).clip_(max_norm)
+    return GradNormPlan(grads, _once=True).clip_(max_norm)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, exp_avg_scales=None, exp_avg_sq_scales=None, **hyper):
     """AdamWPlan(...).step(step, **hyper) in one call."""
-    return AdamWPlan(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales).step(step, **hyper)
+    return AdamWPlan(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, _once=True).step(step, **hyper)

@@ -23,7 +23,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros(())
-    plan = GradNormPlan(grads)
+    plan = GradNormPlan(grads, _once=True)
     _norm_limit(max_norm)
     if error_if_nonfinite:
         norm = plan.norm()
@@ -132,12 +132,12 @@ class AdamW(torch.optim.Optimizer):
         for group, params, grads, states in work:
             keys = ("exp_avg", "exp_avg_sqrt", "exp_avg_scale", "exp_avg_sqrt_scale") if eight else ("exp_avg", "exp_avg_sq")
             plans.append(AdamWPlan(params, grads, *([s[k] for s in states] for k in keys),
-                                   steps=[s["step"] for s in states] if self.capturable else None, _disjoint=True))
+                                   steps=[s["step"] for s in states] if self.capturable else None, _once=True, _disjoint=True))
         max_norm, coef = self.max_norm, None
         self.grad_norm = None
         if max_norm is not None and len(work) > 1:
             # one norm over all groups: its coefficient is left on the device for the groups' calls
-            self.grad_norm, coef = GradNormPlan([g for w in work for g in w[2]]).norm_and_coef(max_norm)
+            self.grad_norm, coef = GradNormPlan([g for w in work for g in w[2]], _once=True).norm_and_coef(max_norm)
             max_norm = None
         for (group, params, _, states), plan in zip(work, plans):
             step = None

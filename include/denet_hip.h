@@ -420,14 +420,21 @@ typedef struct denet_adamw {
                                calls (parameter groups); or NULL.  Not together with max_norm >= 0 */
 } denet_adamw_t;
 int64_t denet_opt_workspace(int64_t count);
-/* norm; and coef for max_norm where asked for */
-int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm /*[1]*/,
-                    float* coef /*[1] or NULL*/, void* ws, int64_t ws_bytes, void* stream);
+/* A device-side table of the list: with it a call is one launch however long the list (without, one for every 52 tensors).
+ * denet_opt_table writes it (denet_opt_table_bytes bytes, 16-byte aligned) and has to be complete before a call
+ * that takes it runs; it holds the addresses, sizes and types of the list and must be written again when any of these change.  step,
+ * step_dev and the hyper-parameters are read from the host structures at every call. */
+int64_t denet_opt_table_bytes(const denet_opt_tensor_t* tensors, int64_t count);
+int denet_opt_table(const denet_opt_tensor_t* tensors, int64_t count, void* table, int64_t table_bytes, void* stream);
+/* norm; and coef for max_norm where asked for.  table: that of `tensors`, or NULL (all calls) */
+int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm,
+                    float* norm /*[1]*/, float* coef /*[1] or NULL*/, void* ws, int64_t ws_bytes, void* stream);
 /* norm, and g <- coef * g in place */
-int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, double max_norm, float* norm /*[1]*/, void* ws,
-                    int64_t ws_bytes, void* stream);
-int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, int bits, const denet_adamw_t* h /* HOST */,
-                     float* norm /*[1], with clipping; else NULL*/, void* ws, int64_t ws_bytes, void* stream);
+int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm,
+                    float* norm /*[1]*/, void* ws, int64_t ws_bytes, void* stream);
+int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, const void* table, int bits,
+                     const denet_adamw_t* h /* HOST */, float* norm /*[1], with clipping; else NULL*/,
+                     void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -65,6 +65,7 @@ def test_norm(sizes, types, offset, dev):
     assert n.dtype == F32 and n.shape == ()
     assert abs(float(n) - want) <= 1.01 * U * want
     assert torch.equal(plan.norm(), n)                                        # same order of sums at every call
+    assert abs(float(ops.grad_norm(grads)) - want) <= 1.01 * U * want         # the list as kernel arguments
     n2, coef = plan.norm_and_coef(0.37 * want)
     assert torch.equal(n2, n) and abs(float(coef) - 0.37) <= (0.37 * 2 * U + 1e-6 / want)
     assert float(plan.norm_and_coef(2.0 * want + 1)[1]) == 1.0
@@ -96,7 +97,7 @@ def test_clip(types, share, dev):
     want = _norm64(grads)
     limit = share * want + (1e-3 if share >= 1 else 0.0)
     versions = [g._version for g in grads]
-    norm = ops.clip_grads_(grads, limit)
+    norm = ops.clip_grads_(grads, limit) if share in (0.25, 3.0) else ops.GradNormPlan(grads).clip_(limit)
     assert abs(float(norm) - want) <= 1.01 * U * want
     c = min(1.0, limit / (want + 1e-6))
     half = 2.0 ** -8
@@ -264,7 +265,7 @@ def test_adamw_one_step(bits, pt, gt, sizes, offset, clip, dev):
     coef = min(1.0, limit / (norm64 + 1e-6)) if clip else 1.0
     t = 7
     versions = [p._version for p in got["p"]]
-    norm = _plan(got, bits).step(t, max_norm=limit if clip else None, **H)
+    norm = _plan(got, bits, _once=len(sizes) > 50).step(t, max_norm=limit if clip else None, **H)
     assert all(p._version > v for p, v in zip(got["p"], versions))
     if clip:
         assert abs(float(norm) - norm64) <= 1.01 * U * norm64
@@ -276,6 +277,21 @@ def test_adamw_one_step(bits, pt, gt, sizes, offset, clip, dev):
             if want is not None:
                 assert _same(got[key][i], want), (key, i, sizes[i])
         _check_64(d, got, i, t, coef, bits, **H)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sizes", [[0, 1, 1025], [5, 300] * 26, [5, 300] * 26 + [7], [0, 19, 5000, 0] * 60])
+def test_lists_with_and_without_a_table(bits, sizes, dev):
+    """A plan (device table, one launch) and the call without one (kernel arguments, a launch for every 52 tensors)."""
+    from denet_amd import ops
+    a = _inputs(sizes, F32, BF16, bits, dev, 33)
+    b, c = _clone(a), _clone(a)
+    _plan(a, bits).step(4, max_norm=1e-3, **H)
+    scales = (b["ms"], b["vs"]) if bits == 8 else (None, None)
+    ops.adamw_step(b["p"], b["g"], b["m"], b["v"], 4, *scales, max_norm=1e-3, **H)
+    _plan(c, bits, _once=True).step([4] * len(sizes), max_norm=1e-3, **H)
+    for key in a:
+        assert all(_same(x, y) and _same(x, z) for x, y, z in zip(a[key], b[key], c[key])), key
 
 
 @pytest.mark.parametrize("bits", [32, 8])

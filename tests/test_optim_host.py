@@ -36,10 +36,10 @@ def test_abi_refuses_bad_gradients(bad):
     lib = _lib.load()
     t = _table([_row(_lib), _row(_lib, **bad)])
     need = _lib.query("denet_opt_workspace", 2)
-    assert lib.denet_grad_norm(ctypes.addressof(t), 2, -1.0, NORM, None, WS, need, None) == BADARG
-    assert lib.denet_grad_clip(ctypes.addressof(t), 2, 1.0, NORM, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(ctypes.addressof(t), 2, None, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_clip(ctypes.addressof(t), 2, None, 1.0, NORM, WS, need, None) == BADARG
     h = _hyper(_lib)
-    assert lib.denet_adamw_step(ctypes.addressof(t), 2, 32, ctypes.addressof(h), None, None, 0, None) == BADARG
+    assert lib.denet_adamw_step(ctypes.addressof(t), 2, None, 32, ctypes.addressof(h), None, None, 0, None) == BADARG
 
 
 def test_abi_refuses_bad_calls():
@@ -47,19 +47,19 @@ def test_abi_refuses_bad_calls():
     lib = _lib.load()
     t = _table([_row(_lib)])
     a, need = ctypes.addressof(t), _lib.query("denet_opt_workspace", 1)
-    assert lib.denet_grad_norm(a, -1, -1.0, NORM, None, WS, need, None) == BADARG
-    assert lib.denet_grad_norm(None, 1, -1.0, NORM, None, WS, need, None) == BADARG
-    assert lib.denet_grad_norm(a, 1, -1.0, None, None, WS, need, None) == BADARG
-    assert lib.denet_grad_norm(a, 1, -1.0, NORM, NORM, WS, need, None) == BADARG            # a coefficient needs max_norm
-    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, None, need, None) == BADARG
-    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, WS + 4, need, None) == BADARG        # workspace alignment
-    assert lib.denet_grad_norm(a, 1, -1.0, NORM, None, WS, need - 1, None) == WORKSPACE
+    assert lib.denet_grad_norm(a, -1, None, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(None, 1, None, -1.0, NORM, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, None, -1.0, None, None, WS, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, None, -1.0, NORM, NORM, WS, need, None) == BADARG            # a coefficient needs max_norm
+    assert lib.denet_grad_norm(a, 1, None, -1.0, NORM, None, None, need, None) == BADARG
+    assert lib.denet_grad_norm(a, 1, None, -1.0, NORM, None, WS + 4, need, None) == BADARG        # workspace alignment
+    assert lib.denet_grad_norm(a, 1, None, -1.0, NORM, None, WS, need - 1, None) == WORKSPACE
     for m in (-1.0, float("nan")):
-        assert lib.denet_grad_clip(a, 1, m, NORM, WS, need, None) == BADARG
+        assert lib.denet_grad_clip(a, 1, None, m, NORM, WS, need, None) == BADARG
     assert _lib.query("denet_opt_workspace", -1) == BADARG
     assert _lib.query("denet_opt_workspace", 0) > 0
     huge = _table([_row(_lib, n=(1 << 48) - 1)])                                            # more chunks than a grid has blocks
-    assert lib.denet_grad_norm(ctypes.addressof(huge), 1, -1.0, NORM, None, WS, need, None) == UNSUPPORTED
+    assert lib.denet_grad_norm(ctypes.addressof(huge), 1, None, -1.0, NORM, None, WS, need, None) == UNSUPPORTED
 
 
 @pytest.mark.parametrize("bits", [8, 32])
@@ -68,9 +68,9 @@ def test_abi_refuses_bad_steps(bits):
     lib = _lib.load()
     need = _lib.query("denet_opt_workspace", 1)
 
-    def call(row={}, norm=None, ws=None, ws_bytes=0, bits=bits, **hyper):
+    def call(row={}, norm=None, ws=None, ws_bytes=0, bits=bits, table=None, **hyper):
         t, h = _table([_row(_lib, **row)]), _hyper(_lib, **hyper)
-        return lib.denet_adamw_step(ctypes.addressof(t), 1, bits, ctypes.addressof(h), norm, ws, ws_bytes, None)
+        return lib.denet_adamw_step(ctypes.addressof(t), 1, table, bits, ctypes.addressof(h), norm, ws, ws_bytes, None)
 
     for row in (dict(param=0), dict(m=0), dict(v=0), dict(param=0x10002), dict(param=0x10001, pt=1), dict(pt=7), dict(step=0), dict(m=0x30002),
                 dict(v=0x40001)):
@@ -81,6 +81,7 @@ def test_abi_refuses_bad_steps(bits):
                   dict(weight_decay=-0.1), dict(max_norm=float("nan"))):
         assert call(**hyper) == BADARG, hyper
     assert call(bits=16) == BADARG
+    assert call(table=0xa0008) == BADARG                                                    # table alignment
     assert call(max_norm=1.0, ws=WS, ws_bytes=need) == BADARG                               # no place for the norm
     assert call(max_norm=1.0, norm=NORM) == BADARG                                          # no workspace
     assert call(max_norm=1.0, norm=NORM, ws=WS, ws_bytes=need - 1) == WORKSPACE
@@ -91,13 +92,27 @@ def test_abi_refuses_bad_steps(bits):
     assert call(dict(step_dev=0x90000), device_steps=1) == BADARG
 
 
+def test_table_refusals():
+    from denet_amd import _lib
+    lib = _lib.load()
+    t = _table([_row(_lib), _row(_lib, n=0)])
+    a = ctypes.addressof(t)
+    need = lib.denet_opt_table_bytes(a, 2)
+    assert need >= 64 + 4 and lib.denet_opt_table_bytes(a, 1) == need
+    assert lib.denet_opt_table_bytes(a, -1) == BADARG and lib.denet_opt_table_bytes(None, 1) == BADARG
+    assert lib.denet_opt_table(a, 2, None, need, None) == BADARG
+    assert lib.denet_opt_table(a, 2, 0xa0008, need, None) == BADARG
+    assert lib.denet_opt_table(a, 2, 0xa0000, need - 1, None) == WORKSPACE
+    assert lib.denet_grad_norm(a, 2, 0xa0008, -1.0, NORM, None, WS, _lib.query("denet_opt_workspace", 2), None) == BADARG
+
+
 def test_nothing_to_do_needs_no_gpu():
     from denet_amd import _lib
     lib = _lib.load()
     h = _hyper(_lib)
     t = _table([_row(_lib, n=0, param=0, grad=0, m=0, v=0, step=0)])
-    assert lib.denet_adamw_step(ctypes.addressof(t), 1, 32, ctypes.addressof(h), None, None, 0, None) == 0
-    assert lib.denet_adamw_step(None, 0, 32, ctypes.addressof(h), None, None, 0, None) == 0
+    assert lib.denet_adamw_step(ctypes.addressof(t), 1, None, 32, ctypes.addressof(h), None, None, 0, None) == 0
+    assert lib.denet_adamw_step(None, 0, None, 32, ctypes.addressof(h), None, None, 0, None) == 0
 
 
 def test_plans_refuse_cpu_tensors_and_empty_lists():
