@@ -18,6 +18,12 @@
 #ifndef NORM_LEAST
 #define NORM_LEAST 4                // least chunks of a block of the norm
 #endif
+#ifndef NT_FROM
+#define NT_FROM (256ll << 20)       // bytes
+#endif
+#ifndef ADAM32_LDS
+#define ADAM32_LDS 44 * 1024
+#endif
 #define E4M3_MAX 448.f
 #define SCALE_MIN 1.1754943508222875e-38f   // 2^-126
 
@@ -25,40 +31,62 @@ typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));      // v
 typedef unsigned short u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 
 // ---- four consecutive elements of a tensor -----------------------------------------------------------------------
+// NT: the streams are larger than the last-level cache and touched once a call, so they pass it by.
+// (not templates of the vector type: a template argument drops its alignment)
+#define LOAD_STORE(V)                                                               \
+    template <bool NT> __device__ __forceinline__ V ld(const V* p) {                \
+        if constexpr (NT) return __builtin_nontemporal_load(p);                     \
+        else return *p;                                                             \
+    }                                                                               \
+    template <bool NT> __device__ __forceinline__ void st(V* p, V v) {              \
+        if constexpr (NT) __builtin_nontemporal_store(v, p);                        \
+        else *p = v;                                                                \
+    }
+LOAD_STORE(f32x4_u)
+LOAD_STORE(u16x4_u)
+LOAD_STORE(unsigned)
+#undef LOAD_STORE
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+// four values to bf16, to nearest even (v_cvt_pk_bf16_f32)
+__device__ __forceinline__ u16x4 to_bf16(const float x[4]) {
+    return __builtin_bit_cast(u16x4, __builtin_convertvector((f32x4{x[0], x[1], x[2], x[3]}), bf16x4));
+}
 template <typename T> struct Quad;
 template <> struct Quad<float> {
-    static __device__ __forceinline__ void load(const float* p, float x[4]) {
-        const f32x4_u v = *reinterpret_cast<const f32x4_u*>(p);
+    template <bool NT> static __device__ __forceinline__ void load(const float* p, float x[4]) {
+        const f32x4_u v = ld<NT>(reinterpret_cast<const f32x4_u*>(p));
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = v[e];
     }
-    static __device__ __forceinline__ void store(float* p, const float x[4]) {
-        *reinterpret_cast<f32x4_u*>(p) = f32x4_u{x[0], x[1], x[2], x[3]};
+    template <bool NT> static __device__ __forceinline__ void store(float* p, const float x[4]) {
+        st<NT>(reinterpret_cast<f32x4_u*>(p), f32x4_u{x[0], x[1], x[2], x[3]});
     }
 };
 template <> struct Quad<unsigned short> {
-    static __device__ __forceinline__ void load(const unsigned short* p, float x[4]) {
-        const u16x4_u v = *reinterpret_cast<const u16x4_u*>(p);
+    template <bool NT> static __device__ __forceinline__ void load(const unsigned short* p, float x[4]) {
+        const u16x4_u v = ld<NT>(reinterpret_cast<const u16x4_u*>(p));
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = bf16_to_f32(v[e]);
     }
-    static __device__ __forceinline__ void store(unsigned short* p, const float x[4]) {
-        *reinterpret_cast<u16x4_u*>(p) = u16x4_u{f32_to_bf16(x[0]), f32_to_bf16(x[1]), f32_to_bf16(x[2]), f32_to_bf16(x[3])};
+    template <bool NT> static __device__ __forceinline__ void store(unsigned short* p, const float x[4]) {
+        st<NT>(reinterpret_cast<u16x4_u*>(p), (u16x4_u)to_bf16(x));
     }
 };
 // k = how many of the four exist (1..4)
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, int k, float x[4]) {
-    if (k == 4) { Quad<T>::load(p, x); return; }
+    if (k == 4) { Quad<T>::template load<false>(p, x); return; }
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = e < k ? FeatIO<T>::load(p + e) : 0.f;
 }
+__device__ __forceinline__ void store_one(float* p, const float x[4], int e) { *p = x[e]; }
+__device__ __forceinline__ void store_one(unsigned short* p, const float x[4], int e) { *p = to_bf16(x)[e]; }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int k, const float x[4]) {
-    if (k == 4) { Quad<T>::store(p, x); return; }
+    if (k == 4) { Quad<T>::template store<false>(p, x); return; }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (e < k) FeatIO<T>::store(p + e, x[e]);
+        if (e < k) store_one(p + e, x, e);
 }
 
 // The argument struct is read where the launch put it: indexing a by-value parameter would copy it to scratch first.
@@ -120,14 +148,14 @@ __device__ __forceinline__ void add_squares(const float x[4], double s[4]) {
 }
 // n consecutive elements by the block; NORM_U loads of a thread in flight
 #define NORM_U 8
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void run_sumsq(const T* g, int64_t n, double s[4]) {
     const int64_t step = 4 * OPT_THREADS;
     int64_t i = 4 * (int)threadIdx.x;
     for (; i + (NORM_U - 1) * step + 4 <= n; i += NORM_U * step) {
         float x[NORM_U][4];
 #pragma unroll
-        for (int u = 0; u < NORM_U; ++u) Quad<T>::load(g + i + u * step, x[u]);
+        for (int u = 0; u < NORM_U; ++u) Quad<T>::template load<NT>(g + i + u * step, x[u]);
 #pragma unroll
         for (int u = 0; u < NORM_U; ++u) add_squares<T>(x[u], s);
     }
@@ -143,7 +171,7 @@ template <typename L> struct NormArgs {
     double* part;
     int chunks;
 };
-template <typename L>
+template <bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs<L> by_value) {
     KARG(NormArgs<L>)& a = *kernel_args<NormArgs<L>>();
     __shared__ double red[4];
@@ -157,8 +185,8 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs<L> by_
         int64_t n = SLOT_N(flags) - first;
         const int64_t most = (int64_t)(end - b) * OPT_CHUNK;
         if (n > most) n = most;
-        if (GRAD_BF16(flags)) run_sumsq((const unsigned short*)t.g + first, n, s);
-        else run_sumsq((const float*)t.g + first, n, s);
+        if (GRAD_BF16(flags)) run_sumsq<NT>((const unsigned short*)t.g + first, n, s);
+        else run_sumsq<NT>((const float*)t.g + first, n, s);
         b += (int)((n + OPT_CHUNK - 1) / OPT_CHUNK);
     }
     const double sum = block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
@@ -190,17 +218,17 @@ template <typename L> struct ScaleArgs {
     ClipArgs clip;
     int first_launch;
 };
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
     float x[OPT_U][4];
     if (left >= OPT_CHUNK) {
 #pragma unroll
-        for (int u = 0; u < OPT_U; ++u) Quad<T>::load(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
+        for (int u = 0; u < OPT_U; ++u) Quad<T>::template load<NT>(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
 #pragma unroll
         for (int u = 0; u < OPT_U; ++u) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[u][e] *= c;
-            Quad<T>::store(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
+            Quad<T>::template store<NT>(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
         }
         return;
     }
@@ -212,7 +240,7 @@ __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
         store4(g + i, k, x[0]);
     }
 }
-template <typename L>
+template <bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by_value) {
     KARG(ScaleArgs<L>)& a = *kernel_args<ScaleArgs<L>>();
     __shared__ double red[4];
@@ -221,8 +249,8 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by
     const int b = blockIdx.x;
     KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
     const int64_t flags = t.n, first = (int64_t)(b - t.start) * OPT_CHUNK, left = SLOT_N(flags) - first;
-    if (GRAD_BF16(flags)) chunk_scale((unsigned short*)t.g + first, left, c);
-    else chunk_scale((float*)t.g + first, left, c);
+    if (GRAD_BF16(flags)) chunk_scale<NT>((unsigned short*)t.g + first, left, c);
+    else chunk_scale<NT>((float*)t.g + first, left, c);
 }
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------
@@ -261,25 +289,25 @@ __device__ __forceinline__ void adam32_quad(float p[4], const float g[4], float 
 }
 
 // a chunk: every load of a thread is requested before the first is used
-template <typename PT, typename GT>
+template <bool NT, typename PT, typename GT>
 __device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float* v, int64_t left, const AdamC& c) {
     float xp[OPT_U][4], xg[OPT_U][4], xm[OPT_U][4], xv[OPT_U][4];
     if (left >= OPT_CHUNK) {
 #pragma unroll
         for (int u = 0; u < OPT_U; ++u) {
             const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
-            Quad<PT>::load(p + i, xp[u]);
-            Quad<GT>::load(g + i, xg[u]);
-            Quad<float>::load(m + i, xm[u]);
-            Quad<float>::load(v + i, xv[u]);
+            Quad<PT>::template load<NT>(p + i, xp[u]);
+            Quad<GT>::template load<NT>(g + i, xg[u]);
+            Quad<float>::load<NT>(m + i, xm[u]);
+            Quad<float>::load<NT>(v + i, xv[u]);
         }
 #pragma unroll
         for (int u = 0; u < OPT_U; ++u) {
             const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
             adam32_quad(xp[u], xg[u], xm[u], xv[u], c);
-            Quad<float>::store(m + i, xm[u]);
-            Quad<float>::store(v + i, xv[u]);
-            Quad<PT>::store(p + i, xp[u]);
+            Quad<float>::store<NT>(m + i, xm[u]);
+            Quad<float>::store<NT>(v + i, xv[u]);
+            Quad<PT>::template store<NT>(p + i, xp[u]);
         }
         return;
     }
@@ -333,20 +361,77 @@ __device__ __forceinline__ void store_codes(unsigned char* p, int k, unsigned w)
     for (int e = 0; e < 3; ++e) if (e < k) p[e] = (unsigned char)(w >> (8 * e));
 }
 
-// maximum over the wave's lanes, in every lane
-__device__ __forceinline__ float wave_max_all(float v) {
-    v = fmaxf(v, dpp_f32<0xB1>(v));      // quad_perm [1,0,3,2]
-    v = fmaxf(v, dpp_f32<0x4E>(v));      // quad_perm [2,3,0,1]
-    v = fmaxf(v, dpp_f32<0x141>(v));     // row_half_mirror
-    v = fmaxf(v, dpp_f32<0x140>(v));     // row_mirror
-    const float r0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0));
-    const float r1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16));
-    const float r2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32));
-    const float r3 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48));
-    return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+// Maximum over the wave of lane values that are >= 0 when read as unsigned, left uniform.
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+#define DPP_MAX(ctrl, rows) do { const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true); v = o > v ? o : v; } while (0)
+    DPP_MAX(0xB1, 0xF);      // quad_perm [1,0,3,2]
+    DPP_MAX(0x4E, 0xF);      // quad_perm [2,3,0,1]
+    DPP_MAX(0x141, 0xF);     // row_half_mirror
+    DPP_MAX(0x140, 0xF);     // row_mirror: every row of 16 lanes has its maximum
+    DPP_MAX(0x142, 0xA);     // row_bcast15 into rows 1 and 3
+    DPP_MAX(0x143, 0xC);     // row_bcast31 into rows 2 and 3
+#undef DPP_MAX
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned umin(unsigned a, unsigned b) { return a < b ? a : b; }
+__device__ __forceinline__ unsigned bits(float x) { return __float_as_uint(x); }
+
+// x / d by the reciprocal and one residual step: the IEEE quotient but for about one pair in 2^30 (then off by one unit in the
+// last place), special operands included; 8 issue slots against 15
+__device__ __forceinline__ float quotient(float x, float d) {
+    const float y = __builtin_amdgcn_rcpf(d), q = x * y;
+    return __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-d, q, x), y, q), d, x);
+}
+// sqrt of 0 or of x in [2^-96, inf): the IEEE result (checked for every mantissa); 9 issue slots against about 20
+__device__ __forceinline__ float root(float x) {
+    const float y = __builtin_amdgcn_rsqf(fmaxf(x, SCALE_MIN)), s = x * y;
+    return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
 }
 
-// four elements of each lane, one QBLOCK of the wave: new moments, the update of p, the codes; -> the two scales
+// The block of adam8_quad for ordinary values, in two thirds of its instructions; false (uniform), and nothing
+// changed, where the wave holds an entry that is not finite or a v in (0, 2^-96).
+// This kernel is bound by instruction issue as much as by memory, so the count is what matters: maxima as unsigned integers (a NaN
+// or an infinity is then the largest, one comparison of the wave's maximum finds it), DPP moves folded into them, rounded-up small
+// codes behind a branch.
+__device__ __forceinline__ bool adam8_ordinary(float p[4], const float g[4], unsigned& mw, unsigned& rw, float& ms, float& rs, const AdamC& c) {
+    float m[4], r[4];
+    from_e4m3x4(mw, ms, m);
+    from_e4m3x4(rw, rs, r);
+    unsigned small = ~0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float v = r[e] * r[e];
+        adam_moments(g[e], m[e], v, c);
+        small = umin(small, bits(v) - 1u);
+        r[e] = root(v);
+    }
+    const unsigned abs = 0x7fffffffu, inf = 0x7f800000u;
+    const unsigned am = wave_max_bits(umax(umax(bits(m[0]) & abs, bits(m[1]) & abs), umax(bits(m[2]) & abs, bits(m[3]) & abs)));
+    const unsigned ar = wave_max_bits(umax(umax(bits(r[0]), bits(r[1])), umax(bits(r[2]), bits(r[3]))));
+    if (am >= inf || ar >= inf || __any(small < 0x0f800000u - 1u)) return false;     // 0x0f800000: 2^-96
+    ms = quant_scale(__uint_as_float(am));
+    rs = quant_scale(__uint_as_float(ar));
+    const float im = quotient(1.f, ms), ir = quotient(1.f, rs);
+    float ym[4], yr[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float denom = r[e] * c.inv_bc2 + c.eps;
+        p[e] = p[e] * c.decay - quotient(m[e], denom) * c.step_size;
+        ym[e] = m[e] * im;
+        yr[e] = r[e] * ir;
+    }
+    if (fminf(fminf(yr[0], yr[1]), fminf(yr[2], yr[3])) < 0.001953125f) {            // 2^-9, the smallest code
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (yr[e] > 0.f && yr[e] < 0.001953125f) yr[e] = 0.001953125f;
+    }
+    mw = e4m3x4(ym);
+    rw = e4m3x4(yr);
+    return true;
+}
+
+// four elements of each lane, one QBLOCK of the wave, any values: new moments, the update of p, the codes; -> the two scales
 __device__ __forceinline__ void adam8_quad(float p[4], const float g[4], unsigned& mw, unsigned& rw, float& ms, float& rs, const AdamC& c) {
     float m[4], r[4];
     from_e4m3x4(mw, ms, m);
@@ -361,8 +446,8 @@ __device__ __forceinline__ void adam8_quad(float p[4], const float g[4], unsigne
         am = fmaxf(am, finite_abs(m[e]));
         ar = fmaxf(ar, finite_abs(r[e]));
     }
-    ms = quant_scale(wave_max_all(am));
-    rs = quant_scale(wave_max_all(ar));
+    ms = quant_scale(__uint_as_float(wave_max_bits(bits(am))));
+    rs = quant_scale(__uint_as_float(wave_max_bits(bits(ar))));
     const float im = 1.f / ms, ir = 1.f / rs;
     float ym[4], yr[4];
 #pragma unroll
@@ -376,7 +461,7 @@ __device__ __forceinline__ void adam8_quad(float p[4], const float g[4], unsigne
 }
 
 // wave w of the block: blocks w, w + 4, ... of the chunk
-template <typename PT, typename GT>
+template <bool NT, typename PT, typename GT>
 __device__ __forceinline__ void adam8_chunk(PT* p, const GT* g, unsigned char* m, unsigned char* r, float* ms, float* rs, int64_t left,
                                             const AdamC& c) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -388,18 +473,18 @@ __device__ __forceinline__ void adam8_chunk(PT* p, const GT* g, unsigned char* m
             const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
             sm[u] = ms[q];
             sr[u] = rs[q];
-            cm[u] = *reinterpret_cast<const unsigned*>(m + i);
-            cr[u] = *reinterpret_cast<const unsigned*>(r + i);
-            Quad<GT>::load(g + i, xg[u]);
-            Quad<PT>::load(p + i, xp[u]);
+            cm[u] = ld<NT>(reinterpret_cast<const unsigned*>(m + i));
+            cr[u] = ld<NT>(reinterpret_cast<const unsigned*>(r + i));
+            Quad<GT>::template load<NT>(g + i, xg[u]);
+            Quad<PT>::template load<NT>(p + i, xp[u]);
         }
 #pragma unroll
         for (int u = 0; u < OPT_U; ++u) {
             const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
-            adam8_quad(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c);
-            *reinterpret_cast<unsigned*>(m + i) = cm[u];
-            *reinterpret_cast<unsigned*>(r + i) = cr[u];
-            Quad<PT>::store(p + i, xp[u]);
+            if (!adam8_ordinary(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c)) adam8_quad(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c);
+            st<NT>(reinterpret_cast<unsigned*>(m + i), cm[u]);
+            st<NT>(reinterpret_cast<unsigned*>(r + i), cr[u]);
+            Quad<PT>::template store<NT>(p + i, xp[u]);
             if (lane == 0) { ms[q] = sm[u]; rs[q] = sr[u]; }
         }
         return;
@@ -428,20 +513,24 @@ __device__ __forceinline__ void adam8_chunk(PT* p, const GT* g, unsigned char* m
     }
 }
 
-template <int BITS, typename PT, typename GT>
+template <int BITS, bool NT, typename PT, typename GT>
 __device__ __forceinline__ void adam_chunk(KARG(Slot)& s, int64_t first, int64_t left, const AdamC& c) {
     if constexpr (BITS == 32)
-        adam32_chunk((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, c);
+        adam32_chunk<NT>((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, c);
     else
-        adam8_chunk((PT*)s.p + first, (const GT*)s.g + first, (unsigned char*)s.m + first, (unsigned char*)s.v + first, s.ms + first / QBLOCK,
+        adam8_chunk<NT>((PT*)s.p + first, (const GT*)s.g + first, (unsigned char*)s.m + first, (unsigned char*)s.v + first, s.ms + first / QBLOCK,
                     s.vs + first / QBLOCK, left, c);
 }
 
-template <int BITS, typename L>
+template <int BITS, bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value) {
     KARG(AdamArgs<L>)& a = *kernel_args<AdamArgs<L>>();
     __shared__ double red[4];
+#ifdef SWZ
+    const int b = xcd_swizzle(blockIdx.x, gridDim.x), i = slot_of(a.list, b);
+#else
     const int b = blockIdx.x, i = slot_of(a.list, b);
+#endif
     KARG(Slot)& s = slot_at(a.list, i);
     const int64_t flags = s.n, first = (int64_t)(b - s.start) * OPT_CHUNK, left = SLOT_N(flags) - first;
     AdamC c = {a.decay, a.b1, a.c1, a.b2, a.c2, a.eps, a.step_size, a.inv_bc2, 1.f};
@@ -454,10 +543,10 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value
     if (a.coef) c.coef = *a.coef;
     if (a.clip.part) c.coef = clip_coef(clip_args(a.clip), red, a.first_launch && b == 0);
     switch ((int)(flags >> 60) & 3) {
-        case 0: adam_chunk<BITS, float, float>(s, first, left, c); break;
-        case 1: adam_chunk<BITS, unsigned short, float>(s, first, left, c); break;
-        case 2: adam_chunk<BITS, float, unsigned short>(s, first, left, c); break;
-        default: adam_chunk<BITS, unsigned short, unsigned short>(s, first, left, c); break;
+        case 0: adam_chunk<BITS, NT, float, float>(s, first, left, c); break;
+        case 1: adam_chunk<BITS, NT, unsigned short, float>(s, first, left, c); break;
+        case 2: adam_chunk<BITS, NT, float, unsigned short>(s, first, left, c); break;
+        default: adam_chunk<BITS, NT, unsigned short, unsigned short>(s, first, left, c); break;
     }
 }
 
@@ -502,18 +591,23 @@ static bool bad_grad(const denet_opt_tensor_t& t) {
     return t.n < 0 || t.n >= (1ll << 48) || (t.n > 0 && !t.grad) || (t.grad_dtype != DENET_F32 && t.grad_dtype != DENET_BF16) ||
            ((uintptr_t)t.grad & (t.grad_dtype == DENET_F32 ? 3 : 1));
 }
-// checks what every call reads; -> the list's chunks and its tensors that have any
-static int check_list(const denet_opt_tensor_t* t, int64_t count, int64_t* chunks_out, int64_t* live_out) {
+// what a call needs to know of the whole list
+struct Facts {
+    int64_t chunks = 0;              // OPT_CHUNKs
+    int64_t live = 0;                // tensors with elements
+    int64_t elements = 0, grad_bytes = 0, param_bytes = 0;
+};
+static int check_list(const denet_opt_tensor_t* t, int64_t count, Facts* f) {
     if (count < 0 || count > (1ll << 24) || (count > 0 && !t)) return DENET_E_BADARG;
-    int64_t chunks = 0, live = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (bad_grad(t[i])) return DENET_E_BADARG;
-        chunks += chunks_of(t[i].n);
-        live += t[i].n > 0;
-        if (chunks >= (1ll << 31)) return DENET_E_UNSUPPORTED;
+        f->chunks += chunks_of(t[i].n);
+        f->live += t[i].n > 0;
+        f->elements += t[i].n;
+        f->grad_bytes += t[i].n * (t[i].grad_dtype == DENET_F32 ? 4 : 2);
+        f->param_bytes += t[i].n * (t[i].param_dtype == DENET_F32 ? 4 : 2);
+        if (f->chunks >= (1ll << 31)) return DENET_E_UNSUPPORTED;
     }
-    *chunks_out = chunks;
-    *live_out = live;
     return DENET_OK;
 }
 static Slot slot_from(const denet_opt_tensor_t& t, int start, int64_t index) {
@@ -547,22 +641,23 @@ static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias 
 static void no_bias(const denet_opt_tensor_t&, float out[2]) { out[0] = out[1] = 0.f; }
 
 // Partial sums of the whole list: at most NORM_PARTS, shared out over the launches by their chunks (rounded up); -> how many were written.
-static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, int64_t total, int64_t live, const void* table, double* part,
-                        hipStream_t st, int* parts_out) {
+static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, hipStream_t st,
+                        int* parts_out) {
     int parts = 0;
+    const bool nt = f.grad_bytes >= NT_FROM;
     auto grid_of = [&](int64_t chunks) {
-        const int64_t most = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (NORM_PARTS - 1) / total + 1;
+        const int64_t most = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (NORM_PARTS - 1) / f.chunks + 1;
         return most < share ? most : share;
     };
     *parts_out = 0;
-    if (!live) return DENET_OK;
+    if (!f.live) return DENET_OK;
     if (table) {
         NormArgs<Tabled> a;
-        a.list = tabled(table, live);
+        a.list = tabled(table, f.live);
         a.part = part;
-        a.chunks = (int)total;
-        parts = (int)grid_of(total);
-        hipLaunchKernelGGL(grad_sumsq_kernel<Tabled>, dim3((unsigned)parts), dim3(OPT_THREADS), 0, st, a);
+        a.chunks = (int)f.chunks;
+        parts = (int)grid_of(f.chunks);
+        hipLaunchKernelGGL((nt ? grad_sumsq_kernel<true, Tabled> : grad_sumsq_kernel<false, Tabled>), dim3((unsigned)parts), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
     } else {
         NormArgs<Packed> a;
@@ -570,7 +665,7 @@ static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, int64_t tota
             const int64_t grid = grid_of(chunks);
             a.part = part + parts;
             a.chunks = chunks;
-            hipLaunchKernelGGL(grad_sumsq_kernel<Packed>, dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+            hipLaunchKernelGGL((nt ? grad_sumsq_kernel<true, Packed> : grad_sumsq_kernel<false, Packed>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
             DENET_CHECK_LAUNCH();
             parts += (int)grid;
             return DENET_OK;
@@ -594,19 +689,20 @@ static int check_ws(const void* ws, int64_t ws_bytes, int64_t count) {
 }
 
 extern "C" int64_t denet_opt_table_bytes(const denet_opt_tensor_t* tensors, int64_t count) {
-    int64_t chunks, live;
-    const int rc = check_list(tensors, count, &chunks, &live);
-    return rc != DENET_OK ? rc : live * (int64_t)sizeof(Slot) + chunks * (int64_t)sizeof(int);
+    Facts f;
+    const int rc = check_list(tensors, count, &f);
+    return rc != DENET_OK ? rc : f.live * (int64_t)sizeof(Slot) + f.chunks * (int64_t)sizeof(int);
 }
 extern "C" int denet_opt_table(const denet_opt_tensor_t* tensors, int64_t count, void* table, int64_t table_bytes, void* stream) {
-    int64_t chunks, live, base = 0, done = 0;
-    int rc = check_list(tensors, count, &chunks, &live);
+    int64_t base = 0, done = 0;
+    Facts f;
+    const int rc = check_list(tensors, count, &f);
     if (rc != DENET_OK) return rc;
     if (!table || ((uintptr_t)table & 15)) return DENET_E_BADARG;
     if (table_bytes < denet_opt_table_bytes(tensors, count)) return DENET_E_WORKSPACE;
     TableArgs a;
     a.slot = (Slot*)table;
-    a.owner = (int*)(a.slot + live);
+    a.owner = (int*)(a.slot + f.live);
     return over_packs(tensors, count, a, no_bias, [&](int n) {
         for (int i = 0; i < a.list.count; ++i) a.list.slot[i].start += (int)done;
         a.chunks = n;
@@ -629,30 +725,31 @@ static int finish_norm(const ClipArgs& c, hipStream_t st) {
 
 extern "C" int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, float* coef,
                                void* ws, int64_t ws_bytes, void* stream) {
-    int64_t chunks, live;
-    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
+    Facts f;
+    int rc = check_list(tensors, count, &f), parts = 0;
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || (coef && !(max_norm >= 0.))) return DENET_E_BADARG;
-    rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, (hipStream_t)stream, &parts);
+    rc = launch_sumsq(tensors, count, f, table, (double*)ws, (hipStream_t)stream, &parts);
     return rc != DENET_OK ? rc : finish_norm({(const double*)ws, max_norm, norm, coef, parts}, (hipStream_t)stream);
 }
 
 extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, void* ws,
                                int64_t ws_bytes, void* stream) {
-    int64_t chunks, live;
-    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
+    Facts f;
+    int rc = check_list(tensors, count, &f), parts = 0;
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || !(max_norm >= 0.)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, st, &parts);
+    rc = launch_sumsq(tensors, count, f, table, (double*)ws, st, &parts);
     if (rc != DENET_OK) return rc;
+    const bool nt = 2 * f.grad_bytes >= NT_FROM;
     const ClipArgs clip = {(const double*)ws, max_norm, norm, nullptr, parts};
-    if (!live) return finish_norm(clip, st);                                   // nothing but empty tensors: norm 0
+    if (!f.live) return finish_norm(clip, st);                                   // nothing but empty tensors: norm 0
     if (table) {
-        const ScaleArgs<Tabled> a = {tabled(table, live), clip, 1};
-        hipLaunchKernelGGL(grad_scale_kernel<Tabled>, dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
+        const ScaleArgs<Tabled> a = {tabled(table, f.live), clip, 1};
+        hipLaunchKernelGGL((nt ? grad_scale_kernel<true, Tabled> : grad_scale_kernel<false, Tabled>), dim3((unsigned)f.chunks), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         return DENET_OK;
     }
@@ -660,7 +757,7 @@ extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count,
     a.clip = clip;
     a.first_launch = 1;
     return over_packs(tensors, count, a, no_bias, [&](int n) {
-        hipLaunchKernelGGL(grad_scale_kernel<Packed>, dim3((unsigned)n), dim3(OPT_THREADS), 0, st, a);
+        hipLaunchKernelGGL((nt ? grad_scale_kernel<true, Packed> : grad_scale_kernel<false, Packed>), dim3((unsigned)n), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         a.first_launch = 0;
         return DENET_OK;
@@ -677,9 +774,10 @@ static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
 }
 
 template <typename L>
-static void launch_adamw(int bits, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
-    if (bits == 8) hipLaunchKernelGGL((adamw_kernel<8, L>), dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
-    else hipLaunchKernelGGL((adamw_kernel<32, L>), dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
+static void launch_adamw(int bits, bool nt, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
+    const dim3 grid((unsigned)chunks), block(OPT_THREADS);
+    if (bits == 8) hipLaunchKernelGGL((nt ? adamw_kernel<8, true, L> : adamw_kernel<8, false, L>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((nt ? adamw_kernel<32, true, L> : adamw_kernel<32, false, L>), grid, block, nt ? ADAM32_LDS : 0, st, a);
 }
 
 extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, const void* table, int bits, const denet_adamw_t* h,
@@ -687,8 +785,8 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     if (!h || bad_table(table) || (bits != 32 && bits != 8)) return DENET_E_BADARG;
     if (!(h->lr >= 0.) || !(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.) ||
         !(h->weight_decay >= 0.) || h->max_norm != h->max_norm) return DENET_E_BADARG;
-    int64_t chunks, live;
-    int rc = check_list(tensors, count, &chunks, &live), parts = 0;
+    Facts f;
+    int rc = check_list(tensors, count, &f), parts = 0;
     if (rc != DENET_OK) return rc;
     bool one_step = true;
     int64_t t_one = 0;
@@ -698,7 +796,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         if (!t_one) t_one = tensors[i].step;
         one_step = one_step && tensors[i].step == t_one;
     }
-    const bool clip = h->max_norm >= 0.;
+    const bool clip = h->max_norm >= 0., nt = 2 * f.param_bytes + f.grad_bytes + f.elements * (bits == 8 ? 4 : 16) >= NT_FROM;
     if (clip || h->device_steps) {
         rc = check_ws(ws, ws_bytes, count);
         if (rc != DENET_OK) return rc;
@@ -707,12 +805,12 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     hipStream_t st = (hipStream_t)stream;
     ClipArgs ca = {nullptr, 0., nullptr, nullptr, 0};
     if (clip) {
-        rc = launch_sumsq(tensors, count, chunks, live, table, (double*)ws, st, &parts);
+        rc = launch_sumsq(tensors, count, f, table, (double*)ws, st, &parts);
         if (rc != DENET_OK) return rc;
         ca = {(const double*)ws, h->max_norm, norm, nullptr, parts};
-        if (!live) return finish_norm(ca, st);
+        if (!f.live) return finish_norm(ca, st);
     }
-    if (!live) return DENET_OK;
+    if (!f.live) return DENET_OK;
     const float* clock = nullptr;
     if (h->device_steps) {
         ClockArgs k;
@@ -754,7 +852,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     if (table && (one_step || h->device_steps)) {
         AdamArgs<Tabled> a;
         fill(a);
-        a.list = tabled(table, live);
+        a.list = tabled(table, f.live);
         if (!h->device_steps) {
             denet_opt_tensor_t t = {};
             t.step = t_one;
@@ -763,14 +861,14 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
             a.step_size = b[0];
             a.inv_bc2 = b[1];
         }
-        launch_adamw(bits, chunks, a, st);
+        launch_adamw(bits, nt, f.chunks, a, st);
         DENET_CHECK_LAUNCH();
         return DENET_OK;
     }
     AdamArgs<Packed> a;
     fill(a);
     return over_packs(tensors, count, a, bias, [&](int n) {
-        launch_adamw(bits, n, a, st);
+        launch_adamw(bits, nt, n, a, st);
         DENET_CHECK_LAUNCH();
         a.first_launch = 0;
         return DENET_OK;
