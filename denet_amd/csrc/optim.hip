@@ -1,28 +1,39 @@
 // Optimizer operators over many tensors at once: the global L2 norm of a gradient list (with its clipping form) and the
 // AdamW step with 32-bit or 8-bit states.
 #include <math.h>
+#include <type_traits>
 #include "denet_common.hpp"
 
 // every operation of this file is rounded by itself (the AdamW step below says why); sums use explicit fma
 #pragma clang fp contract(off)
 
 #define OPT_THREADS 256
-#ifndef OPT_U
-#define OPT_U 1
-#endif
-#define OPT_CHUNK (4 * OPT_U * OPT_THREADS)   // elements of a block: OPT_U vectors of four for each thread
-#define QBLOCK DENET_OPT_QBLOCK     // consecutive elements that share a scale of the 8-bit states (one wave, 4 per lane)
-#ifndef NORM_PARTS
-#define NORM_PARTS 1024             // most partial sums of a norm: every block of the consumer adds them up itself
-#endif
-#ifndef NORM_LEAST
-#define NORM_LEAST 4                // least chunks of a block of the norm
-#endif
+#define ALONE_THREADS 1024
+#define OPT_CHUNK 2048               // elements of a chunk: eight scale blocks, two vectors of four for each thread
+#define QBLOCK DENET_OPT_QBLOCK     // consecutive elements that share a scale of the 8-bit states (32 lanes, 8 each)
 #ifndef NT_FROM
-#define NT_FROM (256ll << 20)       // bytes
+#define NT_FROM (160ll << 20)       // bytes a call streams
 #endif
 #ifndef ADAM32_LDS
 #define ADAM32_LDS 44 * 1024
+#endif
+#ifndef ADAM8_LDS
+#define ADAM8_LDS 44 * 1024
+#endif
+#ifndef NORM_NT_FROM
+#define NORM_NT_FROM (256ll << 20)
+#endif
+#ifndef NORM_PARTS
+#define NORM_PARTS 1024             // most partial sums of a norm
+#endif
+#ifndef NORM_NT_PARTS
+#define NORM_NT_PARTS 256
+#endif
+#ifndef NORM_LEAST
+#define NORM_LEAST 2                // least chunks of a block of the norm
+#endif
+#ifndef NORM_ALONE
+#define NORM_ALONE 32               // most chunks that one block takes alone
 #endif
 #define E4M3_MAX 448.f
 #define SCALE_MIN 1.1754943508222875e-38f   // 2^-126
@@ -133,48 +144,60 @@ __device__ __forceinline__ KARG(Slot)& slot_at(KARG(Tabled)& l, int i) { return 
 // ---- the norm -----------------------------------------------------------------------------------------------------
 // Sums of squares are kept in 64 bits from the first element on: fp32 squares overflow from |g| = 1.8e19 on, and long
 // fp32 sums lose the small gradients.  The fp64 FMA runs at the fp32 rate on this chip, so the pass stays a read.
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    double s = red[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) s += red[w];
+    return s;
 }
 
-template <typename T>
 __device__ __forceinline__ void add_squares(const float x[4], double s[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
 }
 // n consecutive elements by the block; NORM_U loads of a thread in flight
 #define NORM_U 8
-template <bool NT, typename T>
+template <bool NT, int THREADS, typename T>
 __device__ __forceinline__ void run_sumsq(const T* g, int64_t n, double s[4]) {
-    const int64_t step = 4 * OPT_THREADS;
+    const int64_t step = 4 * THREADS;
     int64_t i = 4 * (int)threadIdx.x;
     for (; i + (NORM_U - 1) * step + 4 <= n; i += NORM_U * step) {
         float x[NORM_U][4];
 #pragma unroll
         for (int u = 0; u < NORM_U; ++u) Quad<T>::template load<NT>(g + i + u * step, x[u]);
 #pragma unroll
-        for (int u = 0; u < NORM_U; ++u) add_squares<T>(x[u], s);
+        for (int u = 0; u < NORM_U; ++u) add_squares(x[u], s);
     }
     for (; i < n; i += step) {
         float x[4];
         load4(g + i, n - i < 4 ? (int)(n - i) : 4, x);
-        add_squares<T>(x, s);
+        add_squares(x, s);
     }
+}
+
+// where a norm goes: its value, the clip coefficient for max_norm (each where not NULL)
+struct NormOut { double max_norm; float* norm; float* coef; };
+__device__ __forceinline__ void write_norm(double sum, double max_norm, float* norm, float* coef) {
+    const double n = sqrt(sum), q = max_norm / (n + 1e-6);
+    if (norm) *norm = (float)n;
+    if (coef) *coef = q >= 1. ? 1.f : (float)q;         // a NaN norm makes a NaN coefficient, an infinite one 0
 }
 
 template <typename L> struct NormArgs {
     L list;
-    double* part;
+    double* part;                    // one sum for each block; NULL: the only block writes `out`
+    NormOut out;
     int chunks;
 };
-template <bool NT, typename L>
-__global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs<L> by_value) {
+template <bool NT, int THREADS, typename L>
+__global__ __launch_bounds__(THREADS) void grad_sumsq_kernel(NormArgs<L> by_value) {
     KARG(NormArgs<L>)& a = *kernel_args<NormArgs<L>>();
-    __shared__ double red[4];
+    __shared__ double red[THREADS / 64];
     double s[4] = {0., 0., 0., 0.};
     // a contiguous share of the chunks for each block, walked tensor by tensor
     int b = (int)((int64_t)a.chunks * blockIdx.x / gridDim.x);
@@ -185,47 +208,36 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_sumsq_kernel(NormArgs<L> by_
         int64_t n = SLOT_N(flags) - first;
         const int64_t most = (int64_t)(end - b) * OPT_CHUNK;
         if (n > most) n = most;
-        if (GRAD_BF16(flags)) run_sumsq<NT>((const unsigned short*)t.g + first, n, s);
-        else run_sumsq<NT>((const float*)t.g + first, n, s);
+        if (GRAD_BF16(flags)) run_sumsq<NT, THREADS>((const unsigned short*)t.g + first, n, s);
+        else run_sumsq<NT, THREADS>((const float*)t.g + first, n, s);
         b += (int)((n + OPT_CHUNK - 1) / OPT_CHUNK);
     }
-    const double sum = block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
+    const double sum = block_sum<THREADS>((s[0] + s[1]) + (s[2] + s[3]), red);
+    if (threadIdx.x != 0) return;
+    if (a.part) a.part[blockIdx.x] = sum;
+    else write_norm(sum, a.out.max_norm, a.out.norm, a.out.coef);
 }
 
-struct ClipArgs { const double* part; double max_norm; float* norm; float* coef; int parts; };     // norm, coef: written where not NULL
-
-// every block forms the same sum in the same order
-__device__ __forceinline__ float clip_coef(const ClipArgs& c, double* red, bool write_norm) {
+__global__ __launch_bounds__(OPT_THREADS) void norm_finish_kernel(const double* part, int parts, NormOut out) {
+    __shared__ double red[OPT_THREADS / 64];
     double s = 0.;
-    for (int i = threadIdx.x; i < c.parts; i += OPT_THREADS) s += c.part[i];
-    const double n = sqrt(block_sum(s, red));
-    if (write_norm && threadIdx.x == 0 && c.norm) *c.norm = (float)n;
-    const double q = c.max_norm / (n + 1e-6);
-    const float coef = q >= 1. ? 1.f : (float)q;        // a NaN norm makes a NaN coefficient, an infinite one 0
-    if (write_norm && threadIdx.x == 0 && c.coef) *c.coef = coef;
-    return coef;
-}
-__device__ __forceinline__ ClipArgs clip_args(KARG(ClipArgs)& c) { return {c.part, c.max_norm, c.norm, c.coef, c.parts}; }
-
-__global__ __launch_bounds__(OPT_THREADS) void norm_finish_kernel(ClipArgs c) {
-    __shared__ double red[4];
-    (void)clip_coef(c, red, true);
+    for (int i = threadIdx.x; i < parts; i += OPT_THREADS) s += part[i];
+    s = block_sum<OPT_THREADS>(s, red);
+    if (threadIdx.x == 0) write_norm(s, out.max_norm, out.norm, out.coef);
 }
 
 template <typename L> struct ScaleArgs {
     L list;
-    ClipArgs clip;
-    int first_launch;
+    const float* coef;
 };
 template <bool NT, typename T>
 __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
-    float x[OPT_U][4];
+    float x[2][4];
     if (left >= OPT_CHUNK) {
 #pragma unroll
-        for (int u = 0; u < OPT_U; ++u) Quad<T>::template load<NT>(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
+        for (int u = 0; u < 2; ++u) Quad<T>::template load<NT>(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
 #pragma unroll
-        for (int u = 0; u < OPT_U; ++u) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[u][e] *= c;
             Quad<T>::template store<NT>(g + 4 * (u * OPT_THREADS + (int)threadIdx.x), x[u]);
@@ -243,8 +255,7 @@ __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
 template <bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by_value) {
     KARG(ScaleArgs<L>)& a = *kernel_args<ScaleArgs<L>>();
-    __shared__ double red[4];
-    const float c = clip_coef(clip_args(a.clip), red, a.first_launch && blockIdx.x == 0);
+    const float c = *a.coef;
     if (c == 1.f) return;                               // x * 1 = x for every x
     const int b = blockIdx.x;
     KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
@@ -261,11 +272,9 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by
 struct AdamC { float decay, b1, c1, b2, c2, eps, step_size, inv_bc2, coef; };
 template <typename L> struct AdamArgs {
     L list;
-    ClipArgs clip;                   // clip.part NULL: no clipping
-    const float* coef;               // coefficient that an earlier norm left; or NULL
+    const float* coef;               // multiplies the gradients; or NULL
     const float* clock;              // device-side step counters: decay, then {step_size, inv_bc2} per tensor; or NULL
     float decay, b1, c1, b2, c2, eps, step_size, inv_bc2;
-    int first_launch;
 };
 static_assert(sizeof(AdamArgs<Packed>) <= 4096 && sizeof(ScaleArgs<Packed>) <= 4096 && sizeof(NormArgs<Packed>) <= 4096, "kernel arguments");
 __device__ __forceinline__ void own_bias(KARG(Packed)& l, int i, AdamC& c) { c.step_size = l.bias[i][0]; c.inv_bc2 = l.bias[i][1]; }
@@ -288,39 +297,31 @@ __device__ __forceinline__ void adam32_quad(float p[4], const float g[4], float 
     }
 }
 
-// a chunk: every load of a thread is requested before the first is used
+// half a chunk, one vector of each stream for a thread
+#define HALF (OPT_CHUNK / 2)
 template <bool NT, typename PT, typename GT>
-__device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float* v, int64_t left, const AdamC& c) {
-    float xp[OPT_U][4], xg[OPT_U][4], xm[OPT_U][4], xv[OPT_U][4];
-    if (left >= OPT_CHUNK) {
-#pragma unroll
-        for (int u = 0; u < OPT_U; ++u) {
-            const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
-            Quad<PT>::template load<NT>(p + i, xp[u]);
-            Quad<GT>::template load<NT>(g + i, xg[u]);
-            Quad<float>::load<NT>(m + i, xm[u]);
-            Quad<float>::load<NT>(v + i, xv[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < OPT_U; ++u) {
-            const int i = 4 * (u * OPT_THREADS + (int)threadIdx.x);
-            adam32_quad(xp[u], xg[u], xm[u], xv[u], c);
-            Quad<float>::store<NT>(m + i, xm[u]);
-            Quad<float>::store<NT>(v + i, xv[u]);
-            Quad<PT>::template store<NT>(p + i, xp[u]);
-        }
-        return;
-    }
-    for (int i = 4 * (int)threadIdx.x; i < left; i += 4 * OPT_THREADS) {
+__device__ __forceinline__ void adam32_half(PT* p, const GT* g, float* m, float* v, int64_t left, const AdamC& c) {
+    const int i = 4 * (int)threadIdx.x;
+    float xp[4], xg[4], xm[4], xv[4];
+    if (left >= HALF) {
+        Quad<PT>::template load<NT>(p + i, xp);
+        Quad<GT>::template load<NT>(g + i, xg);
+        Quad<float>::load<NT>(m + i, xm);
+        Quad<float>::load<NT>(v + i, xv);
+        adam32_quad(xp, xg, xm, xv, c);
+        Quad<float>::store<NT>(m + i, xm);
+        Quad<float>::store<NT>(v + i, xv);
+        Quad<PT>::template store<NT>(p + i, xp);
+    } else if (i < left) {
         const int k = left - i < 4 ? (int)(left - i) : 4;
-        load4(p + i, k, xp[0]);
-        load4(g + i, k, xg[0]);
-        load4(m + i, k, xm[0]);
-        load4(v + i, k, xv[0]);
-        adam32_quad(xp[0], xg[0], xm[0], xv[0], c);
-        store4(m + i, k, xm[0]);
-        store4(v + i, k, xv[0]);
-        store4(p + i, k, xp[0]);
+        load4(p + i, k, xp);
+        load4(g + i, k, xg);
+        load4(m + i, k, xm);
+        load4(v + i, k, xv);
+        adam32_quad(xp, xg, xm, xv, c);
+        store4(m + i, k, xm);
+        store4(v + i, k, xv);
+        store4(p + i, k, xp);
     }
 }
 
@@ -332,10 +333,6 @@ __device__ __forceinline__ void adam32_chunk(PT* p, const GT* g, float* m, float
 //  - the update of p uses the moments of this step before they are rounded.
 //  - an entry that is not finite takes the NaN code and is left out of absmax: its neighbours keep their values.
 #define FLOAT_MAX 3.4028234663852886e38f
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = fabsf(x);
-    return a <= FLOAT_MAX ? a : 0.f;
-}
 __device__ __forceinline__ float quant_scale(float amax) {
     const float s = amax * (1.f / E4M3_MAX);
     return s > SCALE_MIN ? s : SCALE_MIN;
@@ -361,17 +358,17 @@ __device__ __forceinline__ void store_codes(unsigned char* p, int k, unsigned w)
     for (int e = 0; e < 3; ++e) if (e < k) p[e] = (unsigned char)(w >> (8 * e));
 }
 
-// Maximum over the wave of lane values that are >= 0 when read as unsigned, left uniform.
-__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
-#define DPP_MAX(ctrl, rows) do { const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true); v = o > v ? o : v; } while (0)
-    DPP_MAX(0xB1, 0xF);      // quad_perm [1,0,3,2]
-    DPP_MAX(0x4E, 0xF);      // quad_perm [2,3,0,1]
-    DPP_MAX(0x141, 0xF);     // row_half_mirror
-    DPP_MAX(0x140, 0xF);     // row_mirror: every row of 16 lanes has its maximum
-    DPP_MAX(0x142, 0xA);     // row_bcast15 into rows 1 and 3
-    DPP_MAX(0x143, 0xC);     // row_bcast31 into rows 2 and 3
+// Maximum over each half of the wave of lane values that are >= 0 when read as unsigned, in every lane.
+__device__ __forceinline__ unsigned half_max_bits(unsigned v) {
+#define DPP_MAX(ctrl) do { const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, true); v = o > v ? o : v; } while (0)
+    DPP_MAX(0xB1);           // quad_perm [1,0,3,2]
+    DPP_MAX(0x4E);           // quad_perm [2,3,0,1]
+    DPP_MAX(0x141);          // row_half_mirror
+    DPP_MAX(0x140);          // row_mirror: every row of 16 lanes has its maximum
 #undef DPP_MAX
-    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+    // exchanges row 1 of one copy with row 0 of the other (3 with 2)
+    const auto two = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return two[0] > two[1] ? two[0] : two[1];
 }
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
 __device__ __forceinline__ unsigned umin(unsigned a, unsigned b) { return a < b ? a : b; }
@@ -389,150 +386,148 @@ __device__ __forceinline__ float root(float x) {
     return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
 }
 
-// The block of adam8_quad for ordinary values, in two thirds of its instructions; false (uniform), and nothing
-// changed, where the wave holds an entry that is not finite or a v in (0, 2^-96).
-// This kernel is bound by instruction issue as much as by memory, so the count is what matters: maxima as unsigned integers (a NaN
-// or an infinity is then the largest, one comparison of the wave's maximum finds it), DPP moves folded into them, rounded-up small
-// codes behind a branch.
-__device__ __forceinline__ bool adam8_ordinary(float p[4], const float g[4], unsigned& mw, unsigned& rw, float& ms, float& rs, const AdamC& c) {
-    float m[4], r[4];
-    from_e4m3x4(mw, ms, m);
-    from_e4m3x4(rw, rs, r);
-    unsigned small = ~0u;
+__device__ __forceinline__ float reciprocal(float s) {               // 1 / s for a normal s with a normal quotient
+    const float y = __builtin_amdgcn_rcpf(s);
+    return __builtin_fmaf(__builtin_fmaf(-s, y, 1.f), y, y);
+}
+#define LEAST 0.001953125f           // 2^-9, the smallest code
+
+// Eight elements of each lane, one QBLOCK for each half of the wave.
+// ORDINARY: for ordinary values, in about 60 % of the instructions; false (uniform), and nothing changed, where the wave holds
+// an entry that is not finite or a v in (0, 2^-96).  This kernel is bound by instruction issue as much as by
+// memory, so the count is what matters: maxima as unsigned integers (a NaN or an infinity is then the largest, one comparison of the
+// maximum finds it), DPP moves folded into them, small codes rounded up behind a branch, two blocks a wave so that
+// the reductions and the scales' arithmetic serve 512 elements.
+template <bool ORDINARY>
+__device__ __forceinline__ bool adam8_blocks(float p[8], const float g[8], unsigned mw[2], unsigned rw[2], float& ms, float& rs, const AdamC& c) {
+    const unsigned inf = 0x7f800000u;
+    float m[8], r[8];
+    from_e4m3x4(mw[0], ms, m);
+    from_e4m3x4(mw[1], ms, m + 4);
+    from_e4m3x4(rw[0], rs, r);
+    from_e4m3x4(rw[1], rs, r + 4);
+    unsigned small = ~0u, am = 0u, ar = 0u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
         float v = r[e] * r[e];
         adam_moments(g[e], m[e], v, c);
-        small = umin(small, bits(v) - 1u);
-        r[e] = root(v);
+        if constexpr (ORDINARY) {
+            small = umin(small, bits(v) - 1u);
+            r[e] = root(v);
+        } else {
+            r[e] = sqrtf(v);
+        }
+        const unsigned bm = bits(m[e]) & 0x7fffffffu, br = bits(r[e]) & (ORDINARY ? ~0u : 0x7fffffffu);
+        am = umax(am, ORDINARY || bm < inf ? bm : 0u);
+        ar = umax(ar, ORDINARY || br < inf ? br : 0u);
     }
-    const unsigned abs = 0x7fffffffu, inf = 0x7f800000u;
-    const unsigned am = wave_max_bits(umax(umax(bits(m[0]) & abs, bits(m[1]) & abs), umax(bits(m[2]) & abs, bits(m[3]) & abs)));
-    const unsigned ar = wave_max_bits(umax(umax(bits(r[0]), bits(r[1])), umax(bits(r[2]), bits(r[3]))));
-    if (am >= inf || ar >= inf || __any(small < 0x0f800000u - 1u)) return false;     // 0x0f800000: 2^-96
+    am = half_max_bits(am);
+    ar = half_max_bits(ar);
+    if (ORDINARY && __any(am >= inf || ar >= inf || small < 0x0f800000u - 1u)) return false;     // 0x0f800000: 2^-96
     ms = quant_scale(__uint_as_float(am));
     rs = quant_scale(__uint_as_float(ar));
-    const float im = quotient(1.f, ms), ir = quotient(1.f, rs);
-    float ym[4], yr[4];
+    const float im = ORDINARY ? reciprocal(ms) : 1.f / ms, ir = ORDINARY ? reciprocal(rs) : 1.f / rs;
+    float ym[8], yr[8], least = 1.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
         const float denom = r[e] * c.inv_bc2 + c.eps;
-        p[e] = p[e] * c.decay - quotient(m[e], denom) * c.step_size;
+        p[e] = p[e] * c.decay - (ORDINARY ? quotient(m[e], denom) : m[e] / denom) * c.step_size;
         ym[e] = m[e] * im;
         yr[e] = r[e] * ir;
+        if constexpr (ORDINARY) {
+            least = fminf(least, yr[e]);
+        } else {
+            if (!(fabsf(m[e]) <= FLOAT_MAX)) ym[e] = __builtin_nanf("");
+            if (!(r[e] <= FLOAT_MAX)) yr[e] = __builtin_nanf("");
+        }
     }
-    if (fminf(fminf(yr[0], yr[1]), fminf(yr[2], yr[3])) < 0.001953125f) {            // 2^-9, the smallest code
+    if (!ORDINARY || least < LEAST) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (yr[e] > 0.f && yr[e] < 0.001953125f) yr[e] = 0.001953125f;
+        for (int e = 0; e < 8; ++e)
+            if (yr[e] > 0.f && yr[e] < LEAST) yr[e] = LEAST;
     }
-    mw = e4m3x4(ym);
-    rw = e4m3x4(yr);
+    mw[0] = e4m3x4(ym);
+    mw[1] = e4m3x4(ym + 4);
+    rw[0] = e4m3x4(yr);
+    rw[1] = e4m3x4(yr + 4);
     return true;
 }
 
-// four elements of each lane, one QBLOCK of the wave, any values: new moments, the update of p, the codes; -> the two scales
-__device__ __forceinline__ void adam8_quad(float p[4], const float g[4], unsigned& mw, unsigned& rw, float& ms, float& rs, const AdamC& c) {
-    float m[4], r[4];
-    from_e4m3x4(mw, ms, m);
-    from_e4m3x4(rw, rs, r);
-    float am = 0.f, ar = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float v = r[e] * r[e];
-        adam_moments(g[e], m[e], v, c);
-        r[e] = sqrtf(v);
-        p[e] = adam_update(p[e], m[e], r[e], c);
-        am = fmaxf(am, finite_abs(m[e]));
-        ar = fmaxf(ar, finite_abs(r[e]));
-    }
-    ms = quant_scale(__uint_as_float(wave_max_bits(bits(am))));
-    rs = quant_scale(__uint_as_float(wave_max_bits(bits(ar))));
-    const float im = 1.f / ms, ir = 1.f / rs;
-    float ym[4], yr[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        ym[e] = fabsf(m[e]) <= FLOAT_MAX ? m[e] * im : __builtin_nanf("");
-        yr[e] = r[e] <= FLOAT_MAX ? r[e] * ir : __builtin_nanf("");
-        if (yr[e] > 0.f && yr[e] < 0.001953125f) yr[e] = 0.001953125f;       // 2^-9, the smallest code
-    }
-    mw = e4m3x4(ym);
-    rw = e4m3x4(yr);
-}
-
-// wave w of the block: blocks w, w + 4, ... of the chunk
+// a chunk: half h of wave w takes scale block 2 w + h, a lane four elements of its first 128 and four of its last
 template <bool NT, typename PT, typename GT>
 __device__ __forceinline__ void adam8_chunk(PT* p, const GT* g, unsigned char* m, unsigned char* r, float* ms, float* rs, int64_t left,
                                             const AdamC& c) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    float xp[OPT_U][4], xg[OPT_U][4], sm[OPT_U], sr[OPT_U];
-    unsigned cm[OPT_U], cr[OPT_U];
+    const int lane = threadIdx.x & 31, q = threadIdx.x >> 5, i = q * QBLOCK + 4 * lane;
+    float xp[8], xg[8], sm, sr;
+    unsigned cm[2], cr[2];
     if (left >= OPT_CHUNK) {
+        sm = ms[q];
+        sr = rs[q];
 #pragma unroll
-        for (int u = 0; u < OPT_U; ++u) {
-            const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
-            sm[u] = ms[q];
-            sr[u] = rs[q];
-            cm[u] = ld<NT>(reinterpret_cast<const unsigned*>(m + i));
-            cr[u] = ld<NT>(reinterpret_cast<const unsigned*>(r + i));
-            Quad<GT>::template load<NT>(g + i, xg[u]);
-            Quad<PT>::template load<NT>(p + i, xp[u]);
+        for (int u = 0; u < 2; ++u) {
+            cm[u] = ld<NT>(reinterpret_cast<const unsigned*>(m + i + 128 * u));
+            cr[u] = ld<NT>(reinterpret_cast<const unsigned*>(r + i + 128 * u));
+            Quad<GT>::template load<NT>(g + i + 128 * u, xg + 4 * u);
+            Quad<PT>::template load<NT>(p + i + 128 * u, xp + 4 * u);
         }
+        if (!adam8_blocks<true>(xp, xg, cm, cr, sm, sr, c)) adam8_blocks<false>(xp, xg, cm, cr, sm, sr, c);
 #pragma unroll
-        for (int u = 0; u < OPT_U; ++u) {
-            const int q = u * (OPT_THREADS / 64) + w, i = q * QBLOCK + 4 * lane;
-            if (!adam8_ordinary(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c)) adam8_quad(xp[u], xg[u], cm[u], cr[u], sm[u], sr[u], c);
-            st<NT>(reinterpret_cast<unsigned*>(m + i), cm[u]);
-            st<NT>(reinterpret_cast<unsigned*>(r + i), cr[u]);
-            Quad<PT>::template store<NT>(p + i, xp[u]);
-            if (lane == 0) { ms[q] = sm[u]; rs[q] = sr[u]; }
+        for (int u = 0; u < 2; ++u) {
+            st<NT>(reinterpret_cast<unsigned*>(m + i + 128 * u), cm[u]);
+            st<NT>(reinterpret_cast<unsigned*>(r + i + 128 * u), cr[u]);
+            Quad<PT>::template store<NT>(p + i + 128 * u, xp + 4 * u);
         }
+        if (lane == 0) { ms[q] = sm; rs[q] = sr; }
         return;
     }
-    for (int q = w; q * QBLOCK < left; q += OPT_THREADS / 64) {
-        const int i = q * QBLOCK + 4 * lane;
-        const int k = left - i >= 4 ? 4 : left > i ? (int)(left - i) : 0;
-        sm[0] = ms[q];
-        sr[0] = rs[q];
-        cm[0] = cr[0] = 0u;
+    const bool live = (int64_t)q * QBLOCK < left;       // (the waves stay whole: the maxima cross lanes)
+    int k[2];
+    sm = live ? ms[q] : 0.f;
+    sr = live ? rs[q] : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) xp[0][e] = xg[0][e] = 0.f;
-        if (k) {
-            load4(p + i, k, xp[0]);
-            load4(g + i, k, xg[0]);
-            cm[0] = load_codes(m + i, k);
-            cr[0] = load_codes(r + i, k);
+    for (int u = 0; u < 2; ++u) {
+        const int at = i + 128 * u;
+        k[u] = left - at >= 4 ? 4 : left > at ? (int)(left - at) : 0;
+        cm[u] = cr[u] = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) xp[4 * u + e] = xg[4 * u + e] = 0.f;
+        if (k[u]) {
+            load4(p + at, k[u], xp + 4 * u);
+            load4(g + at, k[u], xg + 4 * u);
+            cm[u] = load_codes(m + at, k[u]);
+            cr[u] = load_codes(r + at, k[u]);
         }
-        adam8_quad(xp[0], xg[0], cm[0], cr[0], sm[0], sr[0], c);
-        if (k) {
-            store_codes(m + i, k, cm[0]);
-            store_codes(r + i, k, cr[0]);
-            store4(p + i, k, xp[0]);
-        }
-        if (lane == 0) { ms[q] = sm[0]; rs[q] = sr[0]; }
     }
+    adam8_blocks<false>(xp, xg, cm, cr, sm, sr, c);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int at = i + 128 * u;
+        if (!k[u]) continue;
+        store_codes(m + at, k[u], cm[u]);
+        store_codes(r + at, k[u], cr[u]);
+        store4(p + at, k[u], xp + 4 * u);
+    }
+    if (live && lane == 0) { ms[q] = sm; rs[q] = sr; }
 }
 
 template <int BITS, bool NT, typename PT, typename GT>
-__device__ __forceinline__ void adam_chunk(KARG(Slot)& s, int64_t first, int64_t left, const AdamC& c) {
+__device__ __forceinline__ void adam_part(KARG(Slot)& s, int64_t first, int64_t left, const AdamC& c) {
     if constexpr (BITS == 32)
-        adam32_chunk<NT>((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, c);
+        adam32_half<NT>((PT*)s.p + first, (const GT*)s.g + first, (float*)s.m + first, (float*)s.v + first, left, c);
     else
         adam8_chunk<NT>((PT*)s.p + first, (const GT*)s.g + first, (unsigned char*)s.m + first, (unsigned char*)s.v + first, s.ms + first / QBLOCK,
-                    s.vs + first / QBLOCK, left, c);
+                        s.vs + first / QBLOCK, left, c);
 }
 
 template <int BITS, bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value) {
     KARG(AdamArgs<L>)& a = *kernel_args<AdamArgs<L>>();
-    __shared__ double red[4];
-#ifdef SWZ
-    const int b = xcd_swizzle(blockIdx.x, gridDim.x), i = slot_of(a.list, b);
-#else
-    const int b = blockIdx.x, i = slot_of(a.list, b);
-#endif
+    // 8-bit states within the cache: consecutive blocks on one XCD (15.6 against 16.8 us for the 86 MB of the DENet list; streams beyond the
+    // cache 521 against 506 us, 32-bit states 36.4 against 34.5 us the other way)
+    const int id = BITS == 8 && !NT ? xcd_swizzle(blockIdx.x, gridDim.x) : blockIdx.x, b = BITS == 32 ? id >> 1 : id, i = slot_of(a.list, b);
     KARG(Slot)& s = slot_at(a.list, i);
-    const int64_t flags = s.n, first = (int64_t)(b - s.start) * OPT_CHUNK, left = SLOT_N(flags) - first;
+    const int64_t flags = s.n, first = (int64_t)(b - s.start) * OPT_CHUNK + (BITS == 32 ? (id & 1) * HALF : 0), left = SLOT_N(flags) - first;
+    if (left <= 0) return;                              // the last chunk of a tensor may have no second half
     AdamC c = {a.decay, a.b1, a.c1, a.b2, a.c2, a.eps, a.step_size, a.inv_bc2, 1.f};
     own_bias(a.list, i, c);
     if (a.clock) {
@@ -541,12 +536,11 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value
         c.inv_bc2 = a.clock[2 + 2 * s.index];
     }
     if (a.coef) c.coef = *a.coef;
-    if (a.clip.part) c.coef = clip_coef(clip_args(a.clip), red, a.first_launch && b == 0);
     switch ((int)(flags >> 60) & 3) {
-        case 0: adam_chunk<BITS, NT, float, float>(s, first, left, c); break;
-        case 1: adam_chunk<BITS, NT, unsigned short, float>(s, first, left, c); break;
-        case 2: adam_chunk<BITS, NT, float, unsigned short>(s, first, left, c); break;
-        default: adam_chunk<BITS, NT, unsigned short, unsigned short>(s, first, left, c); break;
+        case 0: adam_part<BITS, NT, float, float>(s, first, left, c); break;
+        case 1: adam_part<BITS, NT, unsigned short, float>(s, first, left, c); break;
+        case 2: adam_part<BITS, NT, float, unsigned short>(s, first, left, c); break;
+        default: adam_part<BITS, NT, unsigned short, unsigned short>(s, first, left, c); break;
     }
 }
 
@@ -606,7 +600,7 @@ static int check_list(const denet_opt_tensor_t* t, int64_t count, Facts* f) {
         f->elements += t[i].n;
         f->grad_bytes += t[i].n * (t[i].grad_dtype == DENET_F32 ? 4 : 2);
         f->param_bytes += t[i].n * (t[i].param_dtype == DENET_F32 ? 4 : 2);
-        if (f->chunks >= (1ll << 31)) return DENET_E_UNSUPPORTED;
+        if (f->chunks >= (1ll << 30)) return DENET_E_UNSUPPORTED;
     }
     return DENET_OK;
 }
@@ -640,48 +634,56 @@ static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias 
 }
 static void no_bias(const denet_opt_tensor_t&, float out[2]) { out[0] = out[1] = 0.f; }
 
-// Partial sums of the whole list: at most NORM_PARTS, shared out over the launches by their chunks (rounded up); -> how many were written.
-static int launch_sumsq(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, hipStream_t st,
-                        int* parts_out) {
+// Norm of the whole list into `out`: by one block where the list is short, else partial sums (at most NORM_PARTS, shared out over the
+// launches by their chunks, rounded up) and their sum.
+static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, const NormOut& out, hipStream_t st) {
+    const bool nt = f.grad_bytes >= NORM_NT_FROM;
+    const int64_t most = nt ? NORM_NT_PARTS : NORM_PARTS;
     int parts = 0;
-    const bool nt = f.grad_bytes >= NT_FROM;
     auto grid_of = [&](int64_t chunks) {
-        const int64_t most = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (NORM_PARTS - 1) / f.chunks + 1;
-        return most < share ? most : share;
+        const int64_t full = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (most - 1) / f.chunks + 1;
+        return full < share ? full : share;
     };
-    *parts_out = 0;
-    if (!f.live) return DENET_OK;
-    if (table) {
-        NormArgs<Tabled> a;
-        a.list = tabled(table, f.live);
-        a.part = part;
-        a.chunks = (int)f.chunks;
-        parts = (int)grid_of(f.chunks);
-        hipLaunchKernelGGL((nt ? grad_sumsq_kernel<true, Tabled> : grad_sumsq_kernel<false, Tabled>), dim3((unsigned)parts), dim3(OPT_THREADS), 0, st, a);
+    auto launch = [&](auto& a, int chunks, bool alone) {
+        using L = std::remove_reference_t<decltype(a.list)>;
+        const int64_t grid = alone ? 1 : grid_of(chunks);
+        a.part = alone ? nullptr : part + parts;
+        a.out = out;
+        a.chunks = chunks;
+        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
+        else if (nt) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
-    } else {
-        NormArgs<Packed> a;
-        const int rc = over_packs(t, count, a, no_bias, [&](int chunks) {
-            const int64_t grid = grid_of(chunks);
-            a.part = part + parts;
-            a.chunks = chunks;
-            hipLaunchKernelGGL((nt ? grad_sumsq_kernel<true, Packed> : grad_sumsq_kernel<false, Packed>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
-            DENET_CHECK_LAUNCH();
-            parts += (int)grid;
-            return DENET_OK;
-        });
-        if (rc != DENET_OK) return rc;
+        parts += (int)grid;
+        return DENET_OK;
+    };
+    if (f.live) {
+        const bool alone = f.chunks <= NORM_ALONE && (table || f.live <= PACK);
+        int rc;
+        if (table) {
+            NormArgs<Tabled> a;
+            a.list = tabled(table, f.live);
+            rc = launch(a, (int)f.chunks, alone);
+        } else {
+            NormArgs<Packed> a;
+            rc = over_packs(t, count, a, no_bias, [&](int chunks) { return launch(a, chunks, alone); });
+        }
+        if (rc != DENET_OK || alone) return rc;
     }
-    *parts_out = parts;
+    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(OPT_THREADS), 0, st, (const double*)part, parts, out);
+    DENET_CHECK_LAUNCH();
     return DENET_OK;
 }
 
-// workspace: NORM_PARTS partial sums, one more for each launch (their shares are rounded up); then the clock of device-side counters
+// workspace: NORM_PARTS partial sums, one more for each launch (their shares are rounded up), the coefficient; then the clock of
+// device-side counters
 static int64_t part_bytes(int64_t count) { return (NORM_PARTS + count / PACK + 1) * (int64_t)sizeof(double); }
+static float* coef_in(void* ws, int64_t count) { return (float*)((char*)ws + part_bytes(count)); }
+static float* clock_in(void* ws, int64_t count) { return coef_in(ws, count) + 2; }
 
 extern "C" int64_t denet_opt_workspace(int64_t count) {
     if (count < 0 || count > (1ll << 24)) return DENET_E_BADARG;
-    return part_bytes(count) + (2 * count + 2) * (int64_t)sizeof(float);
+    return part_bytes(count) + (2 * count + 4) * (int64_t)sizeof(float);
 }
 static int check_ws(const void* ws, int64_t ws_bytes, int64_t count) {
     if (!ws || ((uintptr_t)ws & 7)) return DENET_E_BADARG;
@@ -717,51 +719,42 @@ extern "C" int denet_opt_table(const denet_opt_tensor_t* tensors, int64_t count,
 
 static bool bad_table(const void* table) { return (uintptr_t)table & 15; }
 
-static int finish_norm(const ClipArgs& c, hipStream_t st) {
-    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(OPT_THREADS), 0, st, c);
-    DENET_CHECK_LAUNCH();
-    return DENET_OK;
-}
-
 extern "C" int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, float* coef,
                                void* ws, int64_t ws_bytes, void* stream) {
     Facts f;
-    int rc = check_list(tensors, count, &f), parts = 0;
+    int rc = check_list(tensors, count, &f);
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || (coef && !(max_norm >= 0.))) return DENET_E_BADARG;
-    rc = launch_sumsq(tensors, count, f, table, (double*)ws, (hipStream_t)stream, &parts);
-    return rc != DENET_OK ? rc : finish_norm({(const double*)ws, max_norm, norm, coef, parts}, (hipStream_t)stream);
+    return launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef}, (hipStream_t)stream);
 }
 
 extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, void* ws,
                                int64_t ws_bytes, void* stream) {
     Facts f;
-    int rc = check_list(tensors, count, &f), parts = 0;
+    int rc = check_list(tensors, count, &f);
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || !(max_norm >= 0.)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    rc = launch_sumsq(tensors, count, f, table, (double*)ws, st, &parts);
-    if (rc != DENET_OK) return rc;
+    float* coef = coef_in(ws, count);
+    rc = launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef}, st);
+    if (rc != DENET_OK || !f.live) return rc;
     const bool nt = 2 * f.grad_bytes >= NT_FROM;
-    const ClipArgs clip = {(const double*)ws, max_norm, norm, nullptr, parts};
-    if (!f.live) return finish_norm(clip, st);                                   // nothing but empty tensors: norm 0
-    if (table) {
-        const ScaleArgs<Tabled> a = {tabled(table, f.live), clip, 1};
-        hipLaunchKernelGGL((nt ? grad_scale_kernel<true, Tabled> : grad_scale_kernel<false, Tabled>), dim3((unsigned)f.chunks), dim3(OPT_THREADS), 0, st, a);
+    auto launch = [&](auto& a, int chunks) {
+        using L = std::remove_reference_t<decltype(a.list)>;
+        a.coef = coef;
+        hipLaunchKernelGGL((nt ? grad_scale_kernel<true, L> : grad_scale_kernel<false, L>), dim3((unsigned)chunks), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         return DENET_OK;
+    };
+    if (table) {
+        ScaleArgs<Tabled> a;
+        a.list = tabled(table, f.live);
+        return launch(a, (int)f.chunks);
     }
     ScaleArgs<Packed> a;
-    a.clip = clip;
-    a.first_launch = 1;
-    return over_packs(tensors, count, a, no_bias, [&](int n) {
-        hipLaunchKernelGGL((nt ? grad_scale_kernel<true, Packed> : grad_scale_kernel<false, Packed>), dim3((unsigned)n), dim3(OPT_THREADS), 0, st, a);
-        DENET_CHECK_LAUNCH();
-        a.first_launch = 0;
-        return DENET_OK;
-    });
+    return over_packs(tensors, count, a, no_bias, [&](int chunks) { return launch(a, chunks); });
 }
 
 static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
@@ -774,9 +767,9 @@ static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
 }
 
 template <typename L>
-static void launch_adamw(int bits, bool nt, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
-    const dim3 grid((unsigned)chunks), block(OPT_THREADS);
-    if (bits == 8) hipLaunchKernelGGL((nt ? adamw_kernel<8, true, L> : adamw_kernel<8, false, L>), grid, block, 0, st, a);
+static void launch_adamw(int bits, bool nt, bool wide, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
+    const dim3 grid((unsigned)(bits == 8 ? chunks : 2 * chunks)), block(OPT_THREADS);
+    if (bits == 8) hipLaunchKernelGGL((nt ? adamw_kernel<8, true, L> : adamw_kernel<8, false, L>), grid, block, nt && wide ? ADAM8_LDS : 0, st, a);
     else hipLaunchKernelGGL((nt ? adamw_kernel<32, true, L> : adamw_kernel<32, false, L>), grid, block, nt ? ADAM32_LDS : 0, st, a);
 }
 
@@ -786,7 +779,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     if (!(h->lr >= 0.) || !(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.) ||
         !(h->weight_decay >= 0.) || h->max_norm != h->max_norm) return DENET_E_BADARG;
     Facts f;
-    int rc = check_list(tensors, count, &f), parts = 0;
+    int rc = check_list(tensors, count, &f);
     if (rc != DENET_OK) return rc;
     bool one_step = true;
     int64_t t_one = 0;
@@ -803,12 +796,11 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     }
     if ((clip && !norm) || (h->lr_dev && !h->device_steps) || (clip && h->coef)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    ClipArgs ca = {nullptr, 0., nullptr, nullptr, 0};
+    const float* coef = h->coef;
     if (clip) {
-        rc = launch_sumsq(tensors, count, f, table, (double*)ws, st, &parts);
+        rc = launch_norm(tensors, count, f, table, (double*)ws, {h->max_norm, norm, coef_in(ws, count)}, st);
         if (rc != DENET_OK) return rc;
-        ca = {(const double*)ws, h->max_norm, norm, nullptr, parts};
-        if (!f.live) return finish_norm(ca, st);
+        coef = coef_in(ws, count);
     }
     if (!f.live) return DENET_OK;
     const float* clock = nullptr;
@@ -816,7 +808,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         ClockArgs k;
         k.lr = h->lr; k.wd = h->weight_decay; k.b1 = h->beta1; k.b2 = h->beta2;
         k.lr_dev = h->lr_dev;
-        clock = k.clock = (float*)((char*)ws + part_bytes(count));
+        clock = k.clock = clock_in(ws, count);
         for (int64_t i = 0; i < count; i += CLOCK_SLOTS) {
             k.base = (int)i;
             k.count = (int)(count - i < CLOCK_SLOTS ? count - i : CLOCK_SLOTS);
@@ -825,6 +817,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
             DENET_CHECK_LAUNCH();
         }
     }
+    const bool wide = f.param_bytes + f.grad_bytes > 4 * f.elements;           // not both in bf16
     int64_t t_last = 0;
     float bias_last[2] = {0.f, 0.f};
     auto bias = [&](const denet_opt_tensor_t& t, float out[2]) {
@@ -837,8 +830,7 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         out[1] = bias_last[1];
     };
     auto fill = [&](auto& a) {
-        a.clip = ca;
-        a.coef = h->coef;
+        a.coef = coef;
         a.clock = clock;
         a.decay = (float)(1. - h->lr * h->weight_decay);
         a.b1 = (float)h->beta1;
@@ -847,7 +839,6 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         a.c2 = (float)(1. - h->beta2);
         a.eps = (float)h->eps;
         a.step_size = a.inv_bc2 = 0.f;
-        a.first_launch = 1;
     };
     if (table && (one_step || h->device_steps)) {
         AdamArgs<Tabled> a;
@@ -861,16 +852,15 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
             a.step_size = b[0];
             a.inv_bc2 = b[1];
         }
-        launch_adamw(bits, nt, f.chunks, a, st);
+        launch_adamw(bits, nt, wide, f.chunks, a, st);
         DENET_CHECK_LAUNCH();
         return DENET_OK;
     }
     AdamArgs<Packed> a;
     fill(a);
     return over_packs(tensors, count, a, bias, [&](int n) {
-        launch_adamw(bits, nt, n, a, st);
+        launch_adamw(bits, nt, wide, n, a, st);
         DENET_CHECK_LAUNCH();
-        a.first_launch = 0;
         return DENET_OK;
     });
 }

@@ -94,29 +94,18 @@ def _first_device(tensors, what):
     return t.device, t.get_device()
 
 
-class _Table:
-    """The host table of denet_opt_tensor_t rows and the calls on it."""
+class _List:
+    """A host table of denet_opt_tensor_t rows and the calls on it: the list goes to the kernels as launch arguments."""
+    table_addr = None
 
-    def __init__(self, rows, count, device, keep, once):
+    def __init__(self, rows, count, device, index, keep=None):
         self.buf = array.array("q", rows)
         self.addr = self.buf.buffer_info()[0]
         self.count = count
         self.device = device
-        self.index = device.index if device is not None else None
+        self.index = index
         self.keep = keep
         self.ws_bytes = _lib.query("denet_opt_workspace", count)
-        # device-side copy of the list, for plans that are used again: then every call is one launch.  It is complete
-        # when the constructor returns, so the plan may be used on any stream.  (Not while a graph is being captured.)
-        self.table = None
-        if not once and not torch.cuda.is_current_stream_capturing():
-            nbytes = int(_lib.load().denet_opt_table_bytes(self.addr, count))
-            if nbytes > 0:
-                table = torch.empty(nbytes, dtype=torch.uint8, device=device)
-                self._run("denet_opt_table", table.data_ptr(), nbytes)
-                torch.cuda.current_stream(self.index).synchronize()
-                self.table, self.table_addr = table, table.data_ptr()
-        if self.table is None:
-            self.table_addr = None
 
     def ws(self):
         return torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
@@ -130,13 +119,36 @@ class _Table:
 
     def _run(self, name, *args):
         fn = getattr(_lib.load(), name)
-        if self.index != torch.cuda.current_device():
+        if self.index != torch._C._cuda_getDevice():
             with torch.cuda.device(self.index):
                 rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
         else:
             rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
         if rc != 0:
             raise DenetHipError(f"{name} failed: {_lib.strerror(rc)} (code {rc})")
+
+
+class _Table(_List):
+    """The same with a copy of the list on the device, for plans that are used again: every call is then one launch.  The copy is
+    complete when the constructor returns, so the plan may be used on any stream.  (None while a graph is being captured.)"""
+
+    def __init__(self, rows, count, device, index, keep):
+        super().__init__(rows, count, device, index, keep)
+        if not torch.cuda.is_current_stream_capturing():
+            nbytes = int(_lib.load().denet_opt_table_bytes(self.addr, count))
+            if nbytes > 0:
+                table = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                self._run("denet_opt_table", table.data_ptr(), nbytes)
+                torch.cuda.current_stream(index).synchronize()
+                self.table, self.table_addr = table, table.data_ptr()
+        # every call takes a workspace and a scalar of its own from the allocator (empty_like: the call of least host time)
+        self._ws, self._scalar = super().ws(), super().scalar()
+
+    def ws(self):
+        return torch.empty_like(self._ws)
+
+    def scalar(self):
+        return torch.empty_like(self._scalar)
 
 
 def _norm_limit(max_norm):
@@ -159,7 +171,7 @@ class GradNormPlan:
         self.grads = grads
         self._versioned = [g for g in grads if not g.is_inference()]
         self._disjoint = False
-        self._table = _Table(rows, len(grads), device, grads, _once)
+        self._table = (_List if _once else _Table)(rows, len(grads), device, index, grads)
 
     def norm(self):
         """sqrt(sum of squares), accumulated in 64 bits: a 0-d fp32 tensor."""
@@ -189,6 +201,50 @@ class GradNormPlan:
         if self._versioned:
             torch.autograd.graph.increment_version(self._versioned)
         return out
+
+
+def _device_scalar(t, what, device):
+    _check(t, what, (torch.float32,), device)
+    if t.numel() != 1:
+        raise DenetHipError(f"{what}: {t.numel()} values")
+    return t.data_ptr()
+
+
+class _Update:
+    """denet_adamw_step on a list: the hyper-parameters' host structure and the call."""
+
+    def __init__(self, bits, device_steps):
+        self.bits, self.device_steps = bits, device_steps
+        self.h = _lib.AdamWHyper()
+        self.h.device_steps = 1 if device_steps else 0
+        self.addr = ctypes.addressof(self.h)
+
+    def __call__(self, t, lr, betas, eps, weight_decay, max_norm, coef):
+        h = self.h
+        h.lr_dev = h.coef = None
+        if isinstance(lr, torch.Tensor):
+            if not self.device_steps:
+                raise DenetHipError("AdamW: lr as a tensor needs device step counters")
+            h.lr_dev = _device_scalar(lr, "lr", t.device)
+            self.lr = lr
+        else:
+            h.lr = lr
+        h.beta1, h.beta2 = betas
+        h.eps, h.weight_decay = eps, weight_decay
+        if coef is not None:
+            if max_norm is not None:
+                raise DenetHipError("AdamW: max_norm or coef, not both")
+            h.coef = _device_scalar(coef, "coef", t.device)
+        norm, ws = None, None
+        h.max_norm = -1.0
+        if max_norm is not None:
+            h.max_norm = _norm_limit(max_norm)
+            norm = t.scalar()
+        if norm is not None or self.device_steps:
+            ws = t.ws()
+        t.call("denet_adamw_step", self.bits, self.addr, norm.data_ptr() if norm is not None else None,
+               ws.data_ptr() if ws is not None else None, t.ws_bytes if ws is not None else 0)
+        return norm
 
 
 class AdamWPlan:
@@ -243,21 +299,16 @@ class AdamWPlan:
             _check_overlap(written, _spans(grads, at[1]))
         codes = [_CODE[p.dtype] | (_CODE[g.dtype] << 32) for p, g in zip(params, grads)]
         rows = [w for row in zip(at[0], at[1], at[2], at[3], scales[0], scales[1], sizes, [1] * n, counters, codes) for w in row]
-        self.device_steps = steps is not None
         self._versioned = [t for t in params if not t.is_inference()]
-        self._table = _Table(rows, n, device, lists, _once)
-        self._hyper = h = _lib.AdamWHyper()
-        h.device_steps = 1 if self.device_steps else 0
-        self._hyper_addr = ctypes.addressof(h)
-        self._lr = None
+        self._table = (_List if _once else _Table)(rows, n, device, index, lists)
+        self._update = _Update(self.bits, steps is not None)
         self._step = 1
 
     def step(self, step=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, coef=None):
         """One update.  step: the number t >= 1 of this update (an int, or one per parameter); not with device counters.  lr: a number, or (with
         device counters) a one-element fp32 device tensor.  max_norm: clip by the norm of the gradients, which is
         returned (the gradients themselves are not written).  coef: a one-element fp32 device tensor that multiplies the gradients instead."""
-        t, h = self._table, self._hyper
-        if self.device_steps:
+        if self._update.device_steps:
             if step is not None:
                 raise DenetHipError("AdamWPlan.step: this plan counts its steps on the device")
         else:
@@ -267,37 +318,7 @@ class AdamWPlan:
                 raise DenetHipError("AdamWPlan.step: a captured step would repeat its step number at every replay; give the plan "
                                     "device step counters (`steps`)")
             self._set_steps(step)
-        h.lr_dev = None
-        if isinstance(lr, torch.Tensor):
-            if not self.device_steps:
-                raise DenetHipError("AdamWPlan.step: lr as a tensor needs device step counters")
-            _check(lr, "lr", (torch.float32,), t.device)
-            if lr.numel() != 1:
-                raise DenetHipError(f"lr: {lr.numel()} values")
-            h.lr_dev = lr.data_ptr()
-            self._lr = lr
-        else:
-            h.lr = lr
-        h.beta1, h.beta2 = betas
-        h.eps, h.weight_decay = eps, weight_decay
-        h.coef = None
-        if coef is not None:
-            if max_norm is not None:
-                raise DenetHipError("AdamWPlan.step: max_norm or coef, not both")
-            _check(coef, "coef", (torch.float32,), t.device)
-            if coef.numel() != 1:
-                raise DenetHipError(f"coef: {coef.numel()} values")
-            h.coef = coef.data_ptr()
-        norm = ws = None
-        if max_norm is not None:
-            h.max_norm = _norm_limit(max_norm)
-            norm = t.scalar()
-        else:
-            h.max_norm = -1.0
-        if norm is not None or self.device_steps:
-            ws = t.ws()
-        t.call("denet_adamw_step", self.bits, self._hyper_addr, norm.data_ptr() if norm is not None else None,
-               ws.data_ptr() if ws is not None else None, t.ws_bytes if ws is not None else 0)
+        norm = self._update(self._table, lr, betas, eps, weight_decay, max_norm, coef)
         if self._versioned:
             torch.autograd.graph.increment_version(self._versioned)
         return norm

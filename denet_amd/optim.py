@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import DenetHipError
-from .multi_tensor import E4M3, AdamWPlan, GradNormPlan, _check_overlap, _dense, _norm_limit, _spans
+from .multi_tensor import _CODE, E4M3, GradNormPlan, _check_overlap, _dense, _List, _norm_limit, _spans, _Update
 
 __all__ = ["AdamW", "clip_grad_norm_"]
 
@@ -50,6 +50,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.capturable = state_bits, bool(capturable)
         self.max_norm = None if max_norm is None else _norm_limit(max_norm)       # may be changed between steps
         self.grad_norm = None
+        self._update = _Update(state_bits, self.capturable)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     # ---- checks ------------------------------------------------------------------------------
@@ -112,46 +113,82 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
         if capturing and not self.capturable:
             raise DenetHipError("AdamW: a captured step() needs capturable=True (its step numbers would be repeated by every replay)")
-        eight = self.state_bits == 8
-        work = []
+        lists = []
         for group in self.param_groups:
             self._check_group(group)
-            params = [p for p in group["params"] if p.grad is not None]
-            if not params:
-                continue
-            if capturing and any(not self.state[p] for p in params):
-                raise DenetHipError("AdamW: run one eager step before the capture (it creates the state)")
-            work.append((group, params, [self._grad_of(p) for p in params], [self._state_of(p) for p in params]))
-        if not work:
-            self.grad_norm = None
-            return loss
-        plans = []
-        for group, params, grads, states in work:
-            keys = ("exp_avg", "exp_avg_sqrt", "exp_avg_scale", "exp_avg_sqrt_scale") if eight else ("exp_avg", "exp_avg_sq")
-            plans.append(AdamWPlan(params, grads, *([s[k] for s in states] for k in keys),
-                                   steps=[s["step"] for s in states] if self.capturable else None, _once=True, _disjoint=True))
-        max_norm, coef = self.max_norm, None
-        self.grad_norm = None
-        if max_norm is not None and len(work) > 1:
-            # one norm over all groups: its coefficient is left on the device for the groups' calls
-            self.grad_norm, coef = GradNormPlan([g for w in work for g in w[2]], _once=True).norm_and_coef(max_norm)
+            found = self._list_of(group, capturing)
+            if found is not None:
+                lists.append((group, *found))
+        max_norm, coef, self.grad_norm = self.max_norm, None, None
+        if max_norm is not None and len(lists) > 1:
+            # one norm over all groups: its coefficient stays on the device for the groups' calls
+            self.grad_norm, coef = GradNormPlan([g for _, _, _, grads, _ in lists for g in grads], _once=True).norm_and_coef(max_norm)
             max_norm = None
-        for (group, params, _, states), plan in zip(work, plans):
-            step = None
+        for group, table, params, _, states in lists:
+            norm = self._update(table, group["lr"], group["betas"], group["eps"], group["weight_decay"], max_norm, coef)
+            if max_norm is not None:
+                self.grad_norm = norm
             if not self.capturable:
                 for s in states:
                     s["step"] += 1
-                step = [s["step"] for s in states]
-                if min(step) == max(step):
-                    step = step[0]
-            norm = plan.step(step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                             max_norm=max_norm, coef=coef)
-            if max_norm is not None:
-                self.grad_norm = norm
+            torch.autograd.graph.increment_version(params)
         return loss
+
+    def _list_of(self, group, capturing):
+        """(table, parameters, gradients, states) of the group's parameters that have a gradient; None if none has.  Everything the
+        kernels rely on is checked at every step."""
+        state, eight, counted = self.state, self.state_bits == 8, self.capturable
+        k_avg, k_sq = "exp_avg", "exp_avg_sqrt" if eight else "exp_avg_sq"
+        types = {E4M3} if eight else {torch.float32}
+        params, grads, states, rows, index = [], [], [], [], None
+        for p in group["params"]:
+            g = p.grad
+            if g is None:
+                continue
+            s = state[p]
+            if not s:
+                if capturing:
+                    raise DenetHipError("AdamW: run one eager step before the capture (it creates the state)")
+                if not p.is_cuda:
+                    raise DenetHipError("AdamW: parameters must be on a GPU; there is no CPU path")
+                s = self._state_of(p)
+            m, v, n = s[k_avg], s[k_sq], p.numel()
+            if index is None:
+                index, device = p.get_device(), p.device
+            if not (g.layout is torch.strided and g.dtype in _CODE and g.is_contiguous() and p.is_contiguous()):
+                g = self._grad_of(p)
+            # one device, known types, as many elements as the parameter, in the parameter's order
+            if not (p.is_cuda and p.dtype in _CODE and index == p.get_device() == g.get_device() == m.get_device() == v.get_device() and
+                    n == g.numel() == m.numel() == v.numel() and m.dtype in types and v.dtype in types and
+                    (p.is_contiguous() and m.is_contiguous() and v.is_contiguous() or
+                     p.stride() == g.stride() == m.stride() == v.stride() and _dense(p))):
+                raise DenetHipError(f"AdamW: a parameter ({tuple(p.shape)}, {p.dtype}, {p.device}) and its gradient or state do not belong "
+                                    "together, or are not on the GPU of the group's first")
+            ms = vs = step_dev = 0
+            if eight:
+                a, b = s["exp_avg_scale"], s["exp_avg_sqrt_scale"]
+                blocks = -(-n // _lib.OPT_QBLOCK)
+                if not (a.numel() == b.numel() == blocks and a.dtype is b.dtype is torch.float32 and a.is_contiguous() and b.is_contiguous() and
+                        a.get_device() == b.get_device() == index):
+                    raise DenetHipError("AdamW: the scales of a parameter's state do not belong to it")
+                ms, vs = a.data_ptr(), b.data_ptr()
+            if counted:
+                step = s["step"]
+                if not (isinstance(step, torch.Tensor) and step.dtype is torch.int64 and step.get_device() == index and step.numel() == 1):
+                    raise DenetHipError("AdamW: a capturable optimizer counts its steps in one int64 on the device")
+                step_dev, step = step.data_ptr(), 1
+            else:
+                step = s["step"] + 1
+            states.append(s)
+            params.append(p)
+            grads.append(g)
+            rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n, step, step_dev, _CODE[p.dtype] | (_CODE[g.dtype] << 32))
+        if not params:
+            return None
+        return _List(rows, len(params), device, index), params, grads, states
 
     # ---- checkpoints --------------------------------------------------------------------------------
     def load_state_dict(self, state_dict):
@@ -198,7 +235,11 @@ class AdamW(torch.optim.Optimizer):
         out["step"] = torch.full((), step, dtype=torch.int64, device=p.device) if self.capturable else step
         return out
 
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, capturable=self.capturable, max_norm=self.max_norm)
+
     def __setstate__(self, state):
         super().__setstate__(state)
-        for k, v in (("state_bits", 32), ("capturable", False), ("max_norm", None), ("grad_norm", None)):
-            self.__dict__.setdefault(k, v)
+        if "_update" not in self.__dict__:              # a copy or an unpickled one (load_state_dict comes here too)
+            self.grad_norm = None
+            self._update = _Update(self.state_bits, self.capturable)
