@@ -29,6 +29,12 @@
 #ifndef NORM_NT_PARTS
 #define NORM_NT_PARTS 256
 #endif
+#ifndef NORM_G
+#define NORM_G 64
+#endif
+#ifndef ALONE_G
+#define ALONE_G 64
+#endif
 #ifndef NORM_LEAST
 #define NORM_LEAST 2                // least chunks of a block of the norm
 #endif
@@ -40,6 +46,7 @@
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));      // views of a flat bucket start anywhere
 typedef unsigned short u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short u16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 
 // ---- four consecutive elements of a tensor -----------------------------------------------------------------------
 // NT: the streams are larger than the last-level cache and touched once a call, so they pass it by.
@@ -55,6 +62,7 @@ typedef unsigned short u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
     }
 LOAD_STORE(f32x4_u)
 LOAD_STORE(u16x4_u)
+LOAD_STORE(u16x8_u)
 LOAD_STORE(unsigned)
 #undef LOAD_STORE
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -156,28 +164,55 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
     return s;
 }
 
-__device__ __forceinline__ void add_squares(const float x[4], double s[4]) {
+// 16 bytes of a gradient
+template <typename T> struct Line;
+template <> struct Line<float> {
+    static constexpr int N = 4;
+    f32x4_u v;
+    template <bool NT> __device__ __forceinline__ void load(const float* p) { v = ld<NT>(reinterpret_cast<const f32x4_u*>(p)); }
+    __device__ __forceinline__ float at(int e) const { return v[e]; }
+};
+template <> struct Line<unsigned short> {
+    static constexpr int N = 8;
+    u16x8_u v;
+    template <bool NT> __device__ __forceinline__ void load(const unsigned short* p) { v = ld<NT>(reinterpret_cast<const u16x8_u*>(p)); }
+    __device__ __forceinline__ float at(int e) const { return bf16_to_f32(v[e]); }
+};
+template <typename T>
+__device__ __forceinline__ void add_squares(const Line<T>& x, double s[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
+    for (int e = 0; e < Line<T>::N; ++e) s[e & 3] = fma((double)x.at(e), (double)x.at(e), s[e & 3]);
 }
-// n consecutive elements by the block; NORM_U loads of a thread in flight
-#define NORM_U 8
-template <bool NT, int THREADS, typename T>
+// n consecutive elements by a group of G lanes (a wave or the block), U lines of a lane in flight
+template <bool NT, int G, typename T>
 __device__ __forceinline__ void run_sumsq(const T* g, int64_t n, double s[4]) {
-    const int64_t step = 4 * THREADS;
-    int64_t i = 4 * (int)threadIdx.x;
-    for (; i + (NORM_U - 1) * step + 4 <= n; i += NORM_U * step) {
-        float x[NORM_U][4];
+    constexpr int N = Line<T>::N, U = G == 64 ? OPT_CHUNK / (64 * N) : 8;
+    constexpr int64_t step = N * G;
+    int64_t i = N * (int)(threadIdx.x % G);
+    for (; i + (U - 1) * step + N <= n; i += U * step) {
+        Line<T> x[U];
 #pragma unroll
-        for (int u = 0; u < NORM_U; ++u) Quad<T>::template load<NT>(g + i + u * step, x[u]);
+        for (int u = 0; u < U; ++u) x[u].template load<NT>(g + i + u * step);
 #pragma unroll
-        for (int u = 0; u < NORM_U; ++u) add_squares(x[u], s);
+        for (int u = 0; u < U; ++u) add_squares(x[u], s);
     }
-    for (; i < n; i += step) {
-        float x[4];
-        load4(g + i, n - i < 4 ? (int)(n - i) : 4, x);
-        add_squares(x, s);
+    if (i >= n) return;
+    Line<T> x[U];                                       // the rest, all of it in flight too
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t left = n - i - u * step;
+        x[u].v = {};
+        if (left >= N) {
+            x[u].template load<NT>(g + i + u * step);
+        } else if (left > 0) {
+            for (int e = 0; e < (int)left; ++e) {       // the last few elements of a tensor
+                const double y = FeatIO<T>::load(g + i + u * step + e);
+                s[0] = fma(y, y, s[0]);
+            }
+        }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_squares(x[u], s);
 }
 
 // where a norm goes: its value, the clip coefficient for max_norm (each where not NULL)
@@ -194,22 +229,23 @@ template <typename L> struct NormArgs {
     NormOut out;
     int chunks;
 };
-template <bool NT, int THREADS, typename L>
+template <bool NT, int THREADS, int G, typename L>
 __global__ __launch_bounds__(THREADS) void grad_sumsq_kernel(NormArgs<L> by_value) {
     KARG(NormArgs<L>)& a = *kernel_args<NormArgs<L>>();
     __shared__ double red[THREADS / 64];
     double s[4] = {0., 0., 0., 0.};
-    // a contiguous share of the chunks for each block, walked tensor by tensor
-    int b = (int)((int64_t)a.chunks * blockIdx.x / gridDim.x);
-    const int end = (int)((int64_t)a.chunks * (blockIdx.x + 1) / gridDim.x);
+    // a contiguous share of the chunks for each group, walked tensor by tensor
+    const int groups = gridDim.x * (THREADS / G), group = __builtin_amdgcn_readfirstlane(blockIdx.x * (THREADS / G) + threadIdx.x / G);
+    int b = (int)((int64_t)a.chunks * group / groups);
+    const int end = (int)((int64_t)a.chunks * (group + 1) / groups);
     while (b < end) {
         KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
         const int64_t flags = t.n, first = (int64_t)(b - t.start) * OPT_CHUNK;
         int64_t n = SLOT_N(flags) - first;
         const int64_t most = (int64_t)(end - b) * OPT_CHUNK;
         if (n > most) n = most;
-        if (GRAD_BF16(flags)) run_sumsq<NT, THREADS>((const unsigned short*)t.g + first, n, s);
-        else run_sumsq<NT, THREADS>((const float*)t.g + first, n, s);
+        if (GRAD_BF16(flags)) run_sumsq<NT, G>((const unsigned short*)t.g + first, n, s);
+        else run_sumsq<NT, G>((const float*)t.g + first, n, s);
         b += (int)((n + OPT_CHUNK - 1) / OPT_CHUNK);
     }
     const double sum = block_sum<THREADS>((s[0] + s[1]) + (s[2] + s[3]), red);
@@ -650,9 +686,9 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
         a.part = alone ? nullptr : part + parts;
         a.out = out;
         a.chunks = chunks;
-        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
-        else if (nt) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
-        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, ALONE_G, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
+        else if (nt) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, NORM_G, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         parts += (int)grid;
         return DENET_OK;

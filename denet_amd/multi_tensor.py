@@ -2,8 +2,7 @@
 
 A *plan* checks a list of tensors once and holds the table that the library reads at every call, on the host and on the device;
 like a bound step (`_lib.bind`) it keeps the tensors alive, and they stay in place (same storage, type and shape) while it is
-used.  Building one waits for the current stream.  The functions without a plan check the list at every call and hand it over as
-kernel arguments, which takes a launch for every 52 tensors.
+used.  Building one waits for the current stream.  The functions without a plan check and hand over the list at every call.
 
 Tensors are fp32 or bf16, dense (contiguous in some order of their dimensions, all tensors of one parameter in the same order),
 and of one device.  Calls go to torch's current stream of that device; norms are fresh 0-d fp32 tensors, workspaces come from
@@ -94,8 +93,14 @@ def _first_device(tensors, what):
     return t.device, t.get_device()
 
 
+# Lists that are used once go to the kernels as launch arguments, 52 tensors a launch, up to this length; longer ones are
+# written to device memory first, as one launch more.  GPU time of an update of 104 / 110 / 300 tensors of 30 000 elements: 20.7 /
+# 24.9 / 62.6 us as arguments, 21.6 / 24.1 / 58.1 us written; of their norm 8.9 / 11.7 / 28.0 against 9.7 / 11.9 / 20.3 us.
+_ARGUMENTS_UP_TO = 104
+
+
 class _List:
-    """A host table of denet_opt_tensor_t rows and the calls on it: the list goes to the kernels as launch arguments."""
+    """A host table of denet_opt_tensor_t rows and the calls on it."""
     table_addr = None
 
     def __init__(self, rows, count, device, index, keep=None):
@@ -106,12 +111,23 @@ class _List:
         self.index = index
         self.keep = keep
         self.ws_bytes = _lib.query("denet_opt_workspace", count)
+        if count > _ARGUMENTS_UP_TO:
+            self.write_table()
 
     def ws(self):
         return torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
 
     def scalar(self):
         return torch.empty((), dtype=torch.float32, device=self.device)
+
+    def write_table(self):
+        """Puts the list into device memory, in stream order; -> self."""
+        nbytes = int(_lib.load().denet_opt_table_bytes(self.addr, self.count))
+        if nbytes > 0:
+            self.table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            self._run("denet_opt_table", self.table.data_ptr(), nbytes)
+            self.table_addr = self.table.data_ptr()
+        return self
 
     def call(self, name, *args):
         """`args` end before the stream; raw addresses and numbers."""
@@ -130,17 +146,15 @@ class _List:
 
 class _Table(_List):
     """The same with a copy of the list on the device, for plans that are used again: every call is then one launch.  The copy is
-    complete when the constructor returns, so the plan may be used on any stream.  (None while a graph is being captured.)"""
+    complete when the constructor returns, so the plan may be used on any stream.  (While a graph is being captured nothing can be
+    waited for: a plan made then belongs to that graph.)"""
 
     def __init__(self, rows, count, device, index, keep):
         super().__init__(rows, count, device, index, keep)
         if not torch.cuda.is_current_stream_capturing():
-            nbytes = int(_lib.load().denet_opt_table_bytes(self.addr, count))
-            if nbytes > 0:
-                table = torch.empty(nbytes, dtype=torch.uint8, device=device)
-                self._run("denet_opt_table", table.data_ptr(), nbytes)
-                torch.cuda.current_stream(index).synchronize()
-                self.table, self.table_addr = table, table.data_ptr()
+            if self.table_addr is None:
+                self.write_table()
+            torch.cuda.current_stream(index).synchronize()
         # every call takes a workspace and a scalar of its own from the allocator (empty_like: the call of least host time)
         self._ws, self._scalar = super().ws(), super().scalar()
 

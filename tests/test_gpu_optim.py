@@ -322,6 +322,14 @@ def test_adamw_steps_of_their_own(bits, dev):
     d = _clone(got)
     plan.step(9, **H)                                   # and one number for all again
     assert _same(got["p"][1], _same_arithmetic(d, 1, 9, 1.0, bits, **H)[0])
+    n = [33, 0, 2049] * 80                              # in more launches than one
+    d = _inputs(n, F32, F32, bits, dev, 34)
+    got = _clone(d)
+    _plan(got, bits).step([i % 7 + 1 for i in range(len(n))], **H)
+    for i in range(len(n)):
+        if n[i]:
+            want = _same_arithmetic(d, i, i % 7 + 1, 1.0, bits, **H)
+            assert _same(got["p"][i], want[0]) and _same(got["m"][i], want[1]) and _same(got["v"][i], want[2]), i
 
 
 @pytest.mark.parametrize("bits", [32, 8])
