@@ -1,5 +1,11 @@
 // Optimizer operators over many tensors at once: the global L2 norm of a gradient list (with its clipping form) and the
 // AdamW step with 32-bit or 8-bit states.
+//
+// All of them are one pass over their streams.  Measured on one MI355X (three sets of tensors in turn, whole calls):
+//   norm         537 M fp32 elements 305 us = 7.0 TB/s; 161 bf16 tensors, 25 M elements 14.1 us; seven tensors, 0.2 M 10.3 us (two launches)
+//   AdamW, 32    201 M elements 960 us = 5.9 TB/s (a large in-place product reaches 5.9 on this card); 161 tensors with bf16
+//                gradients 113 us = 5.8 TB/s; DENet's 24 tensors, clipped 34 us; seven tensors 6.7 us (host time of one launch)
+//   AdamW, 8     201 M elements 504 us = 6.4 TB/s; 161 bf16 tensors 39.7 us = 5.8 TB/s; DENet's, clipped 23.5 us; seven 6.9 us
 #include <math.h>
 #include <type_traits>
 #include "denet_common.hpp"
@@ -8,39 +14,37 @@
 #pragma clang fp contract(off)
 
 #define OPT_THREADS 256
-#define ALONE_THREADS 1024
-#define OPT_CHUNK 2048               // elements of a chunk: eight scale blocks, two vectors of four for each thread
+#define OPT_CHUNK 2048               // elements of a chunk: eight scale blocks
 #define QBLOCK DENET_OPT_QBLOCK     // consecutive elements that share a scale of the 8-bit states (32 lanes, 8 each)
-#ifndef NT_FROM
-#define NT_FROM (160ll << 20)       // bytes a call streams
-#endif
-#ifndef ADAM32_LDS
-#define ADAM32_LDS 44 * 1024
-#endif
-#ifndef ADAM8_LDS
-#define ADAM8_LDS 44 * 1024
-#endif
-#ifndef NORM_NT_FROM
-#define NORM_NT_FROM (256ll << 20)
-#endif
-#ifndef NORM_PARTS
-#define NORM_PARTS 1024             // most partial sums of a norm
-#endif
-#ifndef NORM_NT_PARTS
-#define NORM_NT_PARTS 256
-#endif
-#ifndef NORM_G
-#define NORM_G 64
-#endif
-#ifndef ALONE_G
-#define ALONE_G 64
-#endif
-#ifndef NORM_LEAST
-#define NORM_LEAST 2                // least chunks of a block of the norm
-#endif
-#ifndef NORM_ALONE
-#define NORM_ALONE 32               // most chunks that one block takes alone
-#endif
+
+// Rules on sizes (256 CUs, 256 MB of last-level cache; times in us on one MI355X, four sets of tensors in turn so that a
+// call does not find its own streams in the cache unless said so).
+//  A step or a scaling that streams at least NT_FROM bytes goes around the cache (non-temporal loads and stores).  AdamW on one fp32 tensor,
+//  cached / around: 100 MB 16.9 / 18.7, 150 MB 29.4 / 26.6, 200 MB 40.8 / 34.4; the same set again and again
+//  250 MB 38.0 / 41.5; scaling in place, 90 MB of gradients 56 / 48.
+#define NT_FROM (160ll << 20)
+//  Those launches keep three blocks on a CU, by asking for LDS that they do not use, where an element is 12 bytes or more: fewer
+//  open streams suit the memory better than more waves (201 M elements, 32-bit states: 8 blocks 1050, 4 blocks 981, 3 blocks 960, 2 blocks
+//  965; 8-bit: 535, 517, 504, -).  All-bf16 8-bit steps are bound by instructions and want the waves (161 tensors:
+//  39.8 at 8 blocks, 47.3 at 3).
+#define NT_LDS (44 * 1024)
+//  A norm whose gradients the same call does not read again goes around the cache from NORM_NT_FROM bytes on, in at most NORM_NT_PARTS blocks
+//  (1 GB fp32: 144.5 at 512 blocks, 146.3 at 256, 146.5 at 1024, cached 169; bf16 146, 188, 150, 171; 60 MB 13.6 against 14.2).  One that
+//  a step or a scaling follows stays cached: 400 MB of gradients clipped in place 186 against 200, 100 M elements' AdamW 529 against 563.
+#define NORM_NT_FROM (64ll << 20)
+#define NORM_NT_PARTS 512
+//  Cached: at most NORM_PARTS blocks of NORM_LEAST chunks or more, a wave walking its own chunks (161 bf16 tensors 14.1; 512 blocks 15.7; the
+//  block walking together, which suits the long runs above, 16.0).
+#define NORM_PARTS 1024
+#define NORM_LEAST 2
+//  Up to NORM_ALONE chunks one block of ALONE_THREADS does it all (65 536 elements: 4.0 of GPU time against 4.9, and a launch
+//  less: 7.1 against 9.7 as called; 131 072: 5.8 against 4.9).
+#define NORM_ALONE 32
+#define ALONE_THREADS 1024
+//  Up to SELF_PARTS partial sums the consumers of the clip coefficient add the sums up themselves, a launch less: clipping the
+//  head's seven tensors in place 10.7 against 13.6 as called.
+#define SELF_PARTS 64
+
 #define E4M3_MAX 448.f
 #define SCALE_MIN 1.1754943508222875e-38f   // 2^-126
 
@@ -217,10 +221,14 @@ __device__ __forceinline__ void run_sumsq(const T* g, int64_t n, double s[4]) {
 
 // where a norm goes: its value, the clip coefficient for max_norm (each where not NULL)
 struct NormOut { double max_norm; float* norm; float* coef; };
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+    const double q = max_norm / (norm + 1e-6);
+    return q >= 1. ? 1.f : (float)q;                    // a NaN norm makes a NaN factor, an infinite one 0
+}
 __device__ __forceinline__ void write_norm(double sum, double max_norm, float* norm, float* coef) {
-    const double n = sqrt(sum), q = max_norm / (n + 1e-6);
+    const double n = sqrt(sum);
     if (norm) *norm = (float)n;
-    if (coef) *coef = q >= 1. ? 1.f : (float)q;         // a NaN norm makes a NaN coefficient, an infinite one 0
+    if (coef) *coef = clip_factor(n, max_norm);
 }
 
 template <typename L> struct NormArgs {
@@ -262,9 +270,29 @@ __global__ __launch_bounds__(OPT_THREADS) void norm_finish_kernel(const double* 
     if (threadIdx.x == 0) write_norm(s, out.max_norm, out.norm, out.coef);
 }
 
+// The clip coefficient as its consumers take it: one number, or the partial sums themselves (one for a lane at most), which every wave
+// adds up in the same order.
+struct Coef {
+    const float* one;                // NULL: take the parts (parts = 0: no clipping)
+    const double* part;
+    double max_norm;
+    float* norm;                     // written by the first block where the parts are taken
+    int parts;
+};
+__device__ __forceinline__ float coef_of(KARG(Coef)& c) {
+    if (c.one) return *c.one;
+    if (!c.parts) return 1.f;
+    const int lane = threadIdx.x & 63;
+    double s = lane < c.parts ? c.part[lane] : 0.;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (blockIdx.x == 0 && threadIdx.x == 0) write_norm(s, c.max_norm, c.norm, nullptr);
+    return clip_factor(sqrt(s), c.max_norm);
+}
+
 template <typename L> struct ScaleArgs {
     L list;
-    const float* coef;
+    Coef coef;
 };
 template <bool NT, typename T>
 __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
@@ -291,7 +319,7 @@ __device__ __forceinline__ void chunk_scale(T* g, int64_t left, float c) {
 template <bool NT, typename L>
 __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by_value) {
     KARG(ScaleArgs<L>)& a = *kernel_args<ScaleArgs<L>>();
-    const float c = *a.coef;
+    const float c = coef_of(a.coef);
     if (c == 1.f) return;                               // x * 1 = x for every x
     const int b = blockIdx.x;
     KARG(Slot)& t = slot_at(a.list, slot_of(a.list, b));
@@ -308,7 +336,7 @@ __global__ __launch_bounds__(OPT_THREADS) void grad_scale_kernel(ScaleArgs<L> by
 struct AdamC { float decay, b1, c1, b2, c2, eps, step_size, inv_bc2, coef; };
 template <typename L> struct AdamArgs {
     L list;
-    const float* coef;               // multiplies the gradients; or NULL
+    Coef coef;                       // multiplies the gradients
     const float* clock;              // device-side step counters: decay, then {step_size, inv_bc2} per tensor; or NULL
     float decay, b1, c1, b2, c2, eps, step_size, inv_bc2;
 };
@@ -333,7 +361,8 @@ __device__ __forceinline__ void adam32_quad(float p[4], const float g[4], float 
     }
 }
 
-// half a chunk, one vector of each stream for a thread
+// Half a chunk: one vector of each stream for a thread, all four in flight (two of each were slower: 201 M elements 1043 us
+// against 960, the DENet list equal).  Bound by memory: seven streams, about 60 instructions an element.
 #define HALF (OPT_CHUNK / 2)
 template <bool NT, typename PT, typename GT>
 __device__ __forceinline__ void adam32_half(PT* p, const GT* g, float* m, float* v, int64_t left, const AdamC& c) {
@@ -431,7 +460,7 @@ __device__ __forceinline__ float reciprocal(float s) {               // 1 / s fo
 // Eight elements of each lane, one QBLOCK for each half of the wave.
 // ORDINARY: for ordinary values, in about 60 % of the instructions; false (uniform), and nothing changed, where the wave holds
 // an entry that is not finite or a v in (0, 2^-96).  This kernel is bound by instruction issue as much as by
-// memory, so the count is what matters: maxima as unsigned integers (a NaN or an infinity is then the largest, one comparison of the
+// memory (299 vector instructions for 512 elements against 626 before), so the count is what matters: maxima as unsigned integers (a NaN or an infinity is then the largest, one comparison of the
 // maximum finds it), DPP moves folded into them, small codes rounded up behind a branch, two blocks a wave so that
 // the reductions and the scales' arithmetic serve 512 elements.
 template <bool ORDINARY>
@@ -563,7 +592,6 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value
     const int id = BITS == 8 && !NT ? xcd_swizzle(blockIdx.x, gridDim.x) : blockIdx.x, b = BITS == 32 ? id >> 1 : id, i = slot_of(a.list, b);
     KARG(Slot)& s = slot_at(a.list, i);
     const int64_t flags = s.n, first = (int64_t)(b - s.start) * OPT_CHUNK + (BITS == 32 ? (id & 1) * HALF : 0), left = SLOT_N(flags) - first;
-    if (left <= 0) return;                              // the last chunk of a tensor may have no second half
     AdamC c = {a.decay, a.b1, a.c1, a.b2, a.c2, a.eps, a.step_size, a.inv_bc2, 1.f};
     own_bias(a.list, i, c);
     if (a.clock) {
@@ -571,7 +599,8 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_kernel(AdamArgs<L> by_value
         c.step_size = a.clock[1 + 2 * s.index];
         c.inv_bc2 = a.clock[2 + 2 * s.index];
     }
-    if (a.coef) c.coef = *a.coef;
+    c.coef = coef_of(a.coef);
+    if (left <= 0) return;                              // the last chunk of a tensor may have no second half
     switch ((int)(flags >> 60) & 3) {
         case 0: adam_part<BITS, NT, float, float>(s, first, left, c); break;
         case 1: adam_part<BITS, NT, unsigned short, float>(s, first, left, c); break;
@@ -602,12 +631,11 @@ __global__ __launch_bounds__(OPT_THREADS) void adamw_clock_kernel(ClockArgs by_v
 }
 
 // ---- the table of a Tabled list: slots, then the owner of every chunk -----------------------------------------------
-struct TableArgs { Packed list; Slot* slot; int* owner; int chunks, base; };
+struct TableArgs { Packed list; Slot* slot; int* owner; int base; };
 static_assert(sizeof(TableArgs) <= 4096, "kernel arguments");
 __global__ __launch_bounds__(OPT_THREADS) void opt_table_kernel(TableArgs by_value) {
     KARG(TableArgs)& a = *kernel_args<TableArgs>();
-    // block i: tensor i of the launch (its chunks are [start, next tensor's start) of the whole list)
-    const int i = blockIdx.x;
+    const int i = blockIdx.x;                           // block i: tensor i of the launch; `start` counts over the whole list
     KARG(Slot)& s = a.list.slot[i];
     if (threadIdx.x == 0) a.slot[a.base + i] = Slot{s.p, s.g, s.m, s.v, s.ms, s.vs, s.n, s.start, s.index};
     const int64_t chunks = (SLOT_N(s.n) + OPT_CHUNK - 1) / OPT_CHUNK;
@@ -636,7 +664,7 @@ static int check_list(const denet_opt_tensor_t* t, int64_t count, Facts* f) {
         f->elements += t[i].n;
         f->grad_bytes += t[i].n * (t[i].grad_dtype == DENET_F32 ? 4 : 2);
         f->param_bytes += t[i].n * (t[i].param_dtype == DENET_F32 ? 4 : 2);
-        if (f->chunks >= (1ll << 30)) return DENET_E_UNSUPPORTED;
+        if (f->chunks >= (1ll << 23)) return DENET_E_UNSUPPORTED;              // a launch has fewer than 2^32 threads
     }
     return DENET_OK;
 }
@@ -647,7 +675,7 @@ static Slot slot_from(const denet_opt_tensor_t& t, int start, int64_t index) {
 
 static Tabled tabled(const void* table, int64_t live) { return {(const Slot*)table, (const int*)((const Slot*)table + live)}; }
 
-// Runs `launch(list, chunks)` over the list: once with its table, or for every PACK tensors.  `bias(i, out)` fills a packed tensor's constants.
+// Fills a.list with PACK tensors at a time and runs `launch(chunks)` for each; `bias(tensor, out)` gives a tensor's constants.
 template <typename Args, typename Bias, typename Launch>
 static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias bias, Launch launch) {
     int64_t chunks = 0;
@@ -671,9 +699,11 @@ static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias 
 static void no_bias(const denet_opt_tensor_t&, float out[2]) { out[0] = out[1] = 0.f; }
 
 // Norm of the whole list into `out`: by one block where the list is short, else partial sums (at most NORM_PARTS, shared out over the
-// launches by their chunks, rounded up) and their sum.
-static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, const NormOut& out, hipStream_t st) {
-    const bool nt = f.grad_bytes >= NORM_NT_FROM;
+// launches by their chunks, rounded up) and their sum.  coef: what the consumers of the coefficient are given.
+static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, const NormOut& out, hipStream_t st,
+                       Coef* coef) {
+    if (coef) *coef = {out.coef, nullptr, 0., nullptr, 0};
+    const bool read_again = out.coef != nullptr, nt = f.grad_bytes >= NORM_NT_FROM && !read_again;
     const int64_t most = nt ? NORM_NT_PARTS : NORM_PARTS;
     int parts = 0;
     auto grid_of = [&](int64_t chunks) {
@@ -686,9 +716,9 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
         a.part = alone ? nullptr : part + parts;
         a.out = out;
         a.chunks = chunks;
-        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, ALONE_G, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
+        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, 64, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
         else if (nt) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
-        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, NORM_G, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, 64, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         parts += (int)grid;
         return DENET_OK;
@@ -705,6 +735,10 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
             rc = over_packs(t, count, a, no_bias, [&](int chunks) { return launch(a, chunks, alone); });
         }
         if (rc != DENET_OK || alone) return rc;
+        if (coef && parts <= SELF_PARTS) {
+            *coef = {nullptr, part, out.max_norm, out.norm, parts};
+            return DENET_OK;
+        }
     }
     hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(OPT_THREADS), 0, st, (const double*)part, parts, out);
     DENET_CHECK_LAUNCH();
@@ -743,7 +777,6 @@ extern "C" int denet_opt_table(const denet_opt_tensor_t* tensors, int64_t count,
     a.owner = (int*)(a.slot + f.live);
     return over_packs(tensors, count, a, no_bias, [&](int n) {
         for (int i = 0; i < a.list.count; ++i) a.list.slot[i].start += (int)done;
-        a.chunks = n;
         a.base = (int)base;
         hipLaunchKernelGGL(opt_table_kernel, dim3((unsigned)a.list.count), dim3(OPT_THREADS), 0, (hipStream_t)stream, a);
         DENET_CHECK_LAUNCH();
@@ -762,7 +795,7 @@ extern "C" int denet_grad_norm(const denet_opt_tensor_t* tensors, int64_t count,
     if (rc == DENET_OK) rc = check_ws(ws, ws_bytes, count);
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || (coef && !(max_norm >= 0.))) return DENET_E_BADARG;
-    return launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef}, (hipStream_t)stream);
+    return launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef}, (hipStream_t)stream, nullptr);
 }
 
 extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count, const void* table, double max_norm, float* norm, void* ws,
@@ -773,8 +806,8 @@ extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count,
     if (rc != DENET_OK) return rc;
     if (!norm || bad_table(table) || !(max_norm >= 0.)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    float* coef = coef_in(ws, count);
-    rc = launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef}, st);
+    Coef coef;
+    rc = launch_norm(tensors, count, f, table, (double*)ws, {max_norm, norm, coef_in(ws, count)}, st, &coef);
     if (rc != DENET_OK || !f.live) return rc;
     const bool nt = 2 * f.grad_bytes >= NT_FROM;
     auto launch = [&](auto& a, int chunks) {
@@ -802,11 +835,13 @@ static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
     return bits == 8 && (!t.avg_scale || !t.sq_scale || ((uintptr_t)t.avg_scale & 3) || ((uintptr_t)t.sq_scale & 3));
 }
 
+// nt: around the cache; wide: an element is 12 bytes or more
 template <typename L>
 static void launch_adamw(int bits, bool nt, bool wide, int64_t chunks, const AdamArgs<L>& a, hipStream_t st) {
     const dim3 grid((unsigned)(bits == 8 ? chunks : 2 * chunks)), block(OPT_THREADS);
-    if (bits == 8) hipLaunchKernelGGL((nt ? adamw_kernel<8, true, L> : adamw_kernel<8, false, L>), grid, block, nt && wide ? ADAM8_LDS : 0, st, a);
-    else hipLaunchKernelGGL((nt ? adamw_kernel<32, true, L> : adamw_kernel<32, false, L>), grid, block, nt ? ADAM32_LDS : 0, st, a);
+    const size_t lds = nt && wide ? NT_LDS : 0;
+    if (bits == 8) hipLaunchKernelGGL((nt ? adamw_kernel<8, true, L> : adamw_kernel<8, false, L>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((nt ? adamw_kernel<32, true, L> : adamw_kernel<32, false, L>), grid, block, lds, st, a);
 }
 
 extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count, const void* table, int bits, const denet_adamw_t* h,
@@ -825,18 +860,18 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         if (!t_one) t_one = tensors[i].step;
         one_step = one_step && tensors[i].step == t_one;
     }
-    const bool clip = h->max_norm >= 0., nt = 2 * f.param_bytes + f.grad_bytes + f.elements * (bits == 8 ? 4 : 16) >= NT_FROM;
+    const int64_t bytes = 2 * f.param_bytes + f.grad_bytes + f.elements * (bits == 8 ? 4 : 16);
+    const bool clip = h->max_norm >= 0., nt = bytes >= NT_FROM, wide = bytes >= 12 * f.elements;
     if (clip || h->device_steps) {
         rc = check_ws(ws, ws_bytes, count);
         if (rc != DENET_OK) return rc;
     }
     if ((clip && !norm) || (h->lr_dev && !h->device_steps) || (clip && h->coef)) return DENET_E_BADARG;
     hipStream_t st = (hipStream_t)stream;
-    const float* coef = h->coef;
+    Coef coef = {h->coef, nullptr, 0., nullptr, 0};
     if (clip) {
-        rc = launch_norm(tensors, count, f, table, (double*)ws, {h->max_norm, norm, coef_in(ws, count)}, st);
+        rc = launch_norm(tensors, count, f, table, (double*)ws, {h->max_norm, norm, coef_in(ws, count)}, st, &coef);
         if (rc != DENET_OK) return rc;
-        coef = coef_in(ws, count);
     }
     if (!f.live) return DENET_OK;
     const float* clock = nullptr;
@@ -853,7 +888,6 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
             DENET_CHECK_LAUNCH();
         }
     }
-    const bool wide = f.param_bytes + f.grad_bytes > 4 * f.elements;           // not both in bf16
     int64_t t_last = 0;
     float bias_last[2] = {0.f, 0.f};
     auto bias = [&](const denet_opt_tensor_t& t, float out[2]) {

@@ -2,7 +2,8 @@
 
 A *plan* checks a list of tensors once and holds the table that the library reads at every call, on the host and on the device;
 like a bound step (`_lib.bind`) it keeps the tensors alive, and they stay in place (same storage, type and shape) while it is
-used.  Building one waits for the current stream.  The functions without a plan check and hand over the list at every call.
+used.  A graph that captured a plan's calls reads the plan's memory: keep the plan as long as the graph.  Building a plan waits for
+the current stream.  The functions without a plan check and hand over the list at every call.
 
 Tensors are fp32 or bf16, dense (contiguous in some order of their dimensions, all tensors of one parameter in the same order),
 and of one device.  Calls go to torch's current stream of that device; norms are fresh 0-d fp32 tensors, workspaces come from
@@ -100,8 +101,8 @@ _ARGUMENTS_UP_TO = 104
 
 
 class _List:
-    """A host table of denet_opt_tensor_t rows and the calls on it."""
-    table_addr = None
+    """A host table of denet_opt_tensor_t rows and the calls on it, all on one stream (a device copy of the table belongs to that stream)."""
+    table = table_addr = None
 
     def __init__(self, rows, count, device, index, keep=None):
         self.buf = array.array("q", rows)
@@ -111,8 +112,11 @@ class _List:
         self.index = index
         self.keep = keep
         self.ws_bytes = _lib.query("denet_opt_workspace", count)
-        if count > _ARGUMENTS_UP_TO:
+        if self.wants_table():
             self.write_table()
+
+    def wants_table(self):
+        return self.count > _ARGUMENTS_UP_TO
 
     def ws(self):
         return torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
@@ -146,23 +150,31 @@ class _List:
 
 class _Table(_List):
     """The same with a copy of the list on the device, for plans that are used again: every call is then one launch.  The copy is
-    complete when the constructor returns, so the plan may be used on any stream.  (While a graph is being captured nothing can be
-    waited for: a plan made then belongs to that graph.)"""
+    complete when the constructor returns, so the plan may be used on any stream.  A plan made while a graph is being captured
+    has none (its memory would be that graph's): its lists stay launch arguments."""
 
     def __init__(self, rows, count, device, index, keep):
         super().__init__(rows, count, device, index, keep)
-        if not torch.cuda.is_current_stream_capturing():
-            if self.table_addr is None:
-                self.write_table()
-            torch.cuda.current_stream(index).synchronize()
+        if self.table is not None:
+            stream = torch.cuda.current_stream(index)
+            stream.synchronize()
+            self.stream = stream.cuda_stream
         # every call takes a workspace and a scalar of its own from the allocator (empty_like: the call of least host time)
         self._ws, self._scalar = super().ws(), super().scalar()
+
+    def wants_table(self):
+        return not torch.cuda.is_current_stream_capturing()
 
     def ws(self):
         return torch.empty_like(self._ws)
 
     def scalar(self):
         return torch.empty_like(self._scalar)
+
+    def call(self, name, *args):
+        if self.table is not None and _lib.current_stream_handle(self.index) != self.stream:
+            self.table.record_stream(torch.cuda.current_stream(self.index))       # the plan may go while that stream still reads it
+        super().call(name, *args)
 
 
 def _norm_limit(max_norm):
@@ -339,7 +351,8 @@ class AdamWPlan:
 
     def _set_steps(self, step):
         t = self._table
-        if isinstance(step, int):
+        if not isinstance(step, (list, tuple)):
+            step = int(step)
             if step != self._step:
                 if step < 1:
                     raise DenetHipError(f"AdamWPlan.step: the first step is 1, got {step}")

@@ -383,7 +383,7 @@ int denet_head_step_train_bwd(const void* Fq, int feat_dtype, const int64_t* lab
  *
  * `tensors` is a HOST array, read during the call (it travels as kernel arguments: nothing is copied to the device, a
  * captured graph holds its own copy).  Tensors with n = 0 are skipped.  param, grad, the 32-bit states and the scales need the alignment of
- * their element, 8-bit codes that of 4 bytes.  No two written ranges may overlap.
+ * their element, 8-bit codes that of 4 bytes.  No two written ranges may overlap.  A list holds fewer than 2^34 elements.
  *
  * bits = 32: exp_avg = m, exp_avg_sq = v, float [n]; avg_scale / sq_scale unused.
  * bits = 8:  exp_avg / exp_avg_sq hold one e4m3 code per element, of m / s and of sqrt(v) / s, with one float s for each

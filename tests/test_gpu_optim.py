@@ -296,7 +296,7 @@ def test_lists_with_and_without_a_table(bits, sizes, dev):
 
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("hyper", [dict(H, weight_decay=0.0), dict(H, betas=(0.0, 0.0)), dict(H, betas=(0.0, 0.99)), dict(H, eps=1e-3),
-                                   dict(H, lr=0.0), dict(H, lr=2.0, weight_decay=0.5)])
+                                   dict(H, lr=0.0), dict(H, lr=2.0, weight_decay=0.5), dict(H, eps=0.0)])
 @pytest.mark.parametrize("t", [1, 2, 1000, 10 ** 7])
 def test_adamw_hyperparameters(bits, hyper, t, dev):
     sizes = [1000, 77]
@@ -588,6 +588,65 @@ def test_streams(dev):
     assert torch.equal(norm, norm2) and torch.equal(got["p"][0], other["p"][0]) and torch.equal(got["v"][0], other["v"][0])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("pt,gt", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
+def test_streams_beyond_the_cache(bits, pt, gt, dev):
+    """Lists whose streams pass the last-level cache by, norms of them alone and with the step that reads the gradients again."""
+    from denet_amd import ops
+    sizes = [22_000_003, 5, 3_000_000, 17_500_001]
+    d = _inputs(sizes, pt, gt, bits, dev, 35, 1)
+    got = _clone(d)
+    norm64 = _norm64(d["g"])
+    assert abs(float(ops.grad_norm(d["g"])) - norm64) <= 1.01 * U * norm64
+    limit = 0.25 * norm64
+    norm = _plan(got, bits).step(3, max_norm=limit, **H)
+    assert abs(float(norm) - norm64) <= 1.01 * U * norm64
+    coef = limit / (norm64 + 1e-6)
+    for i in range(len(sizes)):
+        for key, want in zip(("p", "m", "v", "ms", "vs"), _same_arithmetic(d, i, 3, coef, bits, **H)):
+            assert want is None or _same(got[key][i], want), (key, i)
+    ref = [(g.float() * torch.tensor(coef, dtype=F32, device=dev)).to(g.dtype) for g in d["g"]]
+    ops.clip_grads_(d["g"], limit)
+    assert all(torch.equal(a, b) for a, b in zip(d["g"], ref))
+
+
+def test_a_plan_may_go_while_another_stream_uses_it(dev):
+    from denet_amd import ops
+    g = torch.ones(200_000_000, device=dev)
+    small = [torch.ones(3000, device=dev) for _ in range(60)]
+    plan = ops.GradNormPlan(small + [g])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            norm = plan.norm()
+    del plan
+    fill = [torch.zeros(4_000_000, dtype=torch.uint8, device=dev) for _ in range(50)]      # would take the table's memory
+    torch.cuda.current_stream().wait_stream(s)
+    assert abs(float(norm) - math.sqrt(200_180_000)) <= 1.01 * U * math.sqrt(200_180_000) and len(fill) == 50
+
+
+def test_a_plan_made_during_a_capture(dev):
+    from denet_amd import ops
+    d = _inputs([700, 3] * 80, F32, F32, 32, dev, 36)
+    e = _clone(d)
+    steps = [[torch.zeros((), dtype=torch.int64, device=dev) for _ in d["p"]] for _ in range(2)]
+    ref = _plan(e, 32, steps=steps[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = _plan(d, 32, steps=steps[0])
+        norm = plan.step(**H, max_norm=0.02)
+        n2 = ops.grad_norm(d["g"])
+    for _ in range(3):
+        graph.replay()
+        want = ref.step(**H, max_norm=0.02)
+        assert torch.equal(norm, want) and torch.equal(n2, want)
+        assert all(_same(a, b) for k in ("p", "m", "v") for a, b in zip(d[k], e[k]))
+    plan.step(**H)                                      # and it works outside, too
+    ref.step(**H)
+    assert all(torch.equal(a, b) for a, b in zip(d["p"], e["p"]))
+
+
 def test_long_tensor(dev):
     """Element offsets beyond 2^31 (bytes beyond 2^33): the last elements of a long tensor are stepped and counted."""
     from denet_amd import ops
@@ -706,6 +765,75 @@ def test_optimizer_in_a_graph(bits, dev):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             c = AdamW([b])
             c.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_of_a_long_list_in_a_graph(bits, dev):
+    """More parameters than launch arguments hold; the step's own list is part of the graph."""
+    from denet_amd.optim import AdamW
+    g = _gen(dev, 52)
+    init = [torch.randn(n, device=dev, generator=g) for n in [5, 300, 2049] * 40]
+    a, b = ([torch.nn.Parameter(x.clone()) for x in init] for _ in range(2))
+    oa, ob = AdamW(a, state_bits=bits, capturable=True, max_norm=1.0), AdamW(b, state_bits=bits, max_norm=1.0)
+    for p, q in zip(a, b):
+        p.grad = torch.randn(p.shape, device=dev, generator=g)
+        q.grad = p.grad.clone()
+    oa.step()
+    ob.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for k in range(4):
+        for p, q in zip(a, b):
+            p.grad.copy_(torch.randn(p.shape, device=dev, generator=g))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        ob.step()
+        junk = [torch.full((100_000,), 1e9, device=dev) for _ in range(20)]
+        for p, q in zip(a, b):
+            # (the device's pow may differ from the host's in the last bit of 64: fp32 constants agree but for ties)
+            assert torch.equal(p, q), k
+        del junk
+
+
+def test_copies_of_an_optimizer(dev):
+    import copy
+    from denet_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(500, device=dev))
+    p.grad = torch.ones(500, device=dev)
+    o = AdamW([p], state_bits=8, max_norm=3.0)
+    o.step()
+    q = copy.deepcopy(o)
+    w = q.param_groups[0]["params"][0]
+    assert w is not p and q.max_norm == 3.0 and q.state_bits == 8
+    w.grad = p.grad.clone()
+    o.step()
+    q.step()
+    assert torch.equal(p, w) and q.state[w]["step"] == 2
+
+
+def test_state_that_does_not_fit_is_refused(dev):
+    from denet_amd import _lib
+    from denet_amd.optim import AdamW
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(500, device=dev))
+        o = AdamW([p], state_bits=bits)
+        p.grad = torch.ones(500, device=dev)
+        o.step()
+        keep = p.detach().clone()
+        with torch.no_grad():
+            p.data = torch.ones(700, device=dev)
+        p.grad = torch.ones(700, device=dev)
+        with pytest.raises(_lib.DenetHipError):
+            o.step()                                    # its states are those of 500 elements
+        with torch.no_grad():
+            p.data = keep
+        p.grad = torch.ones(500, device=dev)
+        key = "exp_avg_scale" if bits == 8 else "exp_avg"
+        o.state[p][key] = o.state[p][key].cpu()
+        with pytest.raises(_lib.DenetHipError):
+            o.step()
+        assert torch.equal(p, keep) and o.state[p]["step"] == 1
 
 
 def test_versions_are_seen_by_autograd(dev):
