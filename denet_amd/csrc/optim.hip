@@ -28,11 +28,14 @@
 //  965; 8-bit: 535, 517, 504, -).  All-bf16 8-bit steps are bound by instructions and want the waves (161 tensors:
 //  39.8 at 8 blocks, 47.3 at 3).
 #define NT_LDS (44 * 1024)
-//  A norm whose gradients the same call does not read again goes around the cache from NORM_NT_FROM bytes on, in at most NORM_NT_PARTS blocks
-//  (1 GB fp32: 144.5 at 512 blocks, 146.3 at 256, 146.5 at 1024, cached 169; bf16 146, 188, 150, 171; 60 MB 13.6 against 14.2).  One that
-//  a step or a scaling follows stays cached: 400 MB of gradients clipped in place 186 against 200, 100 M elements' AdamW 529 against 563.
+//  A norm whose gradients the same call does not read again goes around the cache from NORM_NT_FROM bytes on (60 MB 13.6 against 14.2, 1 GB 146
+//  against 169), in 256 blocks for fp32 (5 ragged tensors, 537 M elements: 306 against 319 in 512, one tensor 7.17 against
+//  7.08 TB/s) and 512 with bf16 among it (twice the conversions a byte: 537 M elements 5.3 TB/s in 256, 7.0 in 512, 6.7 in 640).
+//  One that a step or a scaling follows stays cached: 400 MB of gradients clipped in place 186 against 200, 100 M elements' AdamW 529
+//  against 563.
 #define NORM_NT_FROM (64ll << 20)
-#define NORM_NT_PARTS 512
+#define NORM_NT_PARTS 256
+#define NORM_NT_PARTS_BF16 512
 //  Cached: at most NORM_PARTS blocks of NORM_LEAST chunks or more, a wave walking its own chunks (161 bf16 tensors 14.1; 512 blocks 15.7; the
 //  block walking together, which suits the long runs above, 16.0).
 #define NORM_PARTS 1024
@@ -704,7 +707,7 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
                        Coef* coef) {
     if (coef) *coef = {out.coef, nullptr, 0., nullptr, 0};
     const bool read_again = out.coef != nullptr, nt = f.grad_bytes >= NORM_NT_FROM && !read_again;
-    const int64_t most = nt ? NORM_NT_PARTS : NORM_PARTS;
+    const int64_t most = !nt ? NORM_PARTS : f.grad_bytes < 4 * f.elements ? NORM_NT_PARTS_BF16 : NORM_NT_PARTS;
     int parts = 0;
     auto grid_of = [&](int64_t chunks) {
         const int64_t full = (chunks + NORM_LEAST - 1) / NORM_LEAST, share = chunks * (most - 1) / f.chunks + 1;
