@@ -158,7 +158,7 @@ __device__ __forceinline__ KARG(Slot)& slot_at(KARG(Tabled)& l, int i) { return 
 
 // ---- the norm -----------------------------------------------------------------------------------------------------
 // Sums of squares are kept in 64 bits from the first element on: fp32 squares overflow from |g| = 1.8e19 on, and long
-// fp32 sums lose the small gradients.  The fp64 FMA runs at the fp32 rate on this chip, so the pass stays a read.
+// fp32 sums lose the small gradients.  The fp64 FMA runs at the rate of the plain fp32 one on this chip, so the pass stays a read.
 template <int THREADS>
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -463,7 +463,7 @@ __device__ __forceinline__ float reciprocal(float s) {               // 1 / s fo
 // Eight elements of each lane, one QBLOCK for each half of the wave.
 // ORDINARY: for ordinary values, in about 60 % of the instructions; false (uniform), and nothing changed, where the wave holds
 // an entry that is not finite or a v in (0, 2^-96).  This kernel is bound by instruction issue as much as by
-// memory (299 vector instructions for 512 elements against 626 before), so the count is what matters: maxima as unsigned integers (a NaN or an infinity is then the largest, one comparison of the
+// memory (299 vector instructions for 512 elements against 628 at first), so the count is what matters: maxima as unsigned integers (a NaN or an infinity is then the largest, one comparison of the
 // maximum finds it), DPP moves folded into them, small codes rounded up behind a branch, two blocks a wave so that
 // the reductions and the scales' arithmetic serve 512 elements.
 template <bool ORDINARY>

@@ -203,8 +203,9 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the saved parameter groups are not those of an AdamW without amsgrad / maximize")
         by_id = dict(zip((i for g in saved_groups for i in g["params"]), (p for g in self.param_groups for p in g["params"])))
         fresh = {p: self._converted(p, saved[i]) for i, p in by_id.items() if i in saved and saved[i]}
-        super().load_state_dict({"state": {}, "param_groups": [{k: v for k, v in g.items() if k in ("params", "initial_lr") or k in self.defaults}
-                                                               for g in saved_groups]})
+        # (a scheduler's own entries stay; the flags of torch's class have no meaning here)
+        flags = ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay")
+        super().load_state_dict({"state": {}, "param_groups": [{k: v for k, v in g.items() if k not in flags} for g in saved_groups]})
         for p, s in fresh.items():
             self.state[p] = s
 

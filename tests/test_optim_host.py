@@ -186,6 +186,15 @@ def test_load_state_dict_refuses_other_optimizers():
     again = AdamW([p], state_bits=32)
     again.load_state_dict(opt.state_dict())
     assert torch.equal(again.state[p]["exp_avg"], s["exp_avg"]) and again.state[p]["step"] == 2
+    sched = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=1.0, total_steps=10, cycle_momentum=False)
+    kept = opt.state_dict()
+    again.load_state_dict(kept)
+    assert all(again.param_groups[0][k] == v for k, v in kept["param_groups"][0].items()) and "max_lr" in again.param_groups[0] and sched
+    import copy
+    import pickle
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):                     # (this test's own bytes)
+        assert other.state_bits == 32 and not other.capturable and other.max_norm is None
+        assert torch.equal(next(iter(other.state.values()))["exp_avg"], s["exp_avg"])
     half = torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))
     kept = AdamW([half])
     kept.load_state_dict(opt.state_dict())
