@@ -199,7 +199,7 @@ class AdamW(torch.optim.Optimizer):
                                                               for a, b in zip(saved_groups, self.param_groups)):
             raise ValueError("the saved state has other parameter groups than this optimizer")
         for g in saved_groups:
-            if not all(k in g for k in self.defaults) or g.get("amsgrad") or g.get("maximize"):
+            if not all(k in g for k in ("lr", "betas", "eps", "weight_decay")) or g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("the saved parameter groups are not those of an AdamW without amsgrad / maximize")
         by_id = dict(zip((i for g in saved_groups for i in g["params"]), (p for g in self.param_groups for p in g["params"])))
         fresh = {p: self._converted(p, saved[i]) for i, p in by_id.items() if i in saved and saved[i]}
