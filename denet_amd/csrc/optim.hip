@@ -2,7 +2,7 @@
 // AdamW step with 32-bit or 8-bit states.
 //
 // All of them are one pass over their streams.  Measured on one MI355X (three sets of tensors in turn, whole calls):
-//   norm         537 M fp32 elements 305 us = 7.0 TB/s; 161 bf16 tensors, 25 M elements 14.1 us; seven tensors, 0.2 M 10.3 us (two launches)
+//   norm         537 M fp32 elements 305 us = 7.0 TB/s; 161 bf16 tensors, 25 M elements 14.0 us; seven tensors, 0.2 M 10.7 us (two launches)
 //   AdamW, 32    201 M elements 960 us = 5.9 TB/s (a large in-place product reaches 5.9 on this card); 161 tensors with bf16
 //                gradients 113 us = 5.8 TB/s; DENet's 24 tensors, clipped 34 us; seven tensors 6.7 us (host time of one launch)
 //   AdamW, 8     201 M elements 504 us = 6.4 TB/s; 161 bf16 tensors 39.7 us = 5.8 TB/s; DENet's, clipped 23.5 us; seven 6.9 us
@@ -35,15 +35,16 @@
 //  against 563.
 #define NORM_NT_FROM (64ll << 20)
 #define NORM_NT_PARTS 256
-#define NORM_NT_PARTS_BF16 512
-//  Cached: at most NORM_PARTS blocks of NORM_LEAST chunks or more, a wave walking its own chunks (161 bf16 tensors 14.1; 512 blocks 15.7; the
-//  block walking together, which suits the long runs above, 16.0).
-#define NORM_PARTS 1024
-#define NORM_LEAST 2
-//  Up to NORM_ALONE chunks one block of ALONE_THREADS does it all (65 536 elements: 4.0 of GPU time against 4.9, and a launch
-//  less: 7.1 against 9.7 as called; 131 072: 5.8 against 4.9).
+#define NORM_NT_PARTS_BF16 512      // (the most partial sums of any norm)
+//  Cached: at most NORM_PARTS blocks of NORM_LEAST chunks or more, a wave walking its own chunks (161 bf16 tensors 14.4; the block
+//  walking together, which suits the long runs above, 16.0).  Blocks of 1024 threads: the same waves in 1024 blocks of 256 take 19.1 against
+//  18.1 for clipping the DENet list in place, 34.4 against 33.0 for its clipped step, 14.3 against 14.5 for the 161 tensors.
+#define NORM_THREADS 1024
+#define NORM_PARTS 256
+#define NORM_LEAST 4
+//  Up to NORM_ALONE chunks one block does it all (65 536 elements: 4.0 of GPU time against 4.9, and a launch less: 7.1 against 9.7 as
+//  called; 131 072: 5.8 against 4.9).
 #define NORM_ALONE 32
-#define ALONE_THREADS 1024
 //  Up to SELF_PARTS partial sums the consumers of the clip coefficient add the sums up themselves, a launch less: clipping the
 //  head's seven tensors in place 10.7 against 13.6 as called.
 #define SELF_PARTS 64
@@ -286,7 +287,8 @@ __device__ __forceinline__ float coef_of(KARG(Coef)& c) {
     if (c.one) return *c.one;
     if (!c.parts) return 1.f;
     const int lane = threadIdx.x & 63;
-    double s = lane < c.parts ? c.part[lane] : 0.;
+    double s = 0.;
+    for (int i = lane; i < c.parts; i += 64) s += c.part[i];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if (blockIdx.x == 0 && threadIdx.x == 0) write_norm(s, c.max_norm, c.norm, nullptr);
@@ -701,7 +703,7 @@ static int over_packs(const denet_opt_tensor_t* t, int64_t count, Args& a, Bias 
 }
 static void no_bias(const denet_opt_tensor_t&, float out[2]) { out[0] = out[1] = 0.f; }
 
-// Norm of the whole list into `out`: by one block where the list is short, else partial sums (at most NORM_PARTS, shared out over the
+// Norm of the whole list into `out`: by one block where the list is short, else partial sums (at most NORM_NT_PARTS_BF16, shared out over the
 // launches by their chunks, rounded up) and their sum.  coef: what the consumers of the coefficient are given.
 static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& f, const void* table, double* part, const NormOut& out, hipStream_t st,
                        Coef* coef) {
@@ -719,9 +721,8 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
         a.part = alone ? nullptr : part + parts;
         a.out = out;
         a.chunks = chunks;
-        if (alone) hipLaunchKernelGGL((grad_sumsq_kernel<false, ALONE_THREADS, 64, L>), dim3(1), dim3(ALONE_THREADS), 0, st, a);
-        else if (nt) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
-        else hipLaunchKernelGGL((grad_sumsq_kernel<false, OPT_THREADS, 64, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        if (nt && !alone) hipLaunchKernelGGL((grad_sumsq_kernel<true, OPT_THREADS, OPT_THREADS, L>), dim3((unsigned)grid), dim3(OPT_THREADS), 0, st, a);
+        else hipLaunchKernelGGL((grad_sumsq_kernel<false, NORM_THREADS, 64, L>), dim3((unsigned)grid), dim3(NORM_THREADS), 0, st, a);
         DENET_CHECK_LAUNCH();
         parts += (int)grid;
         return DENET_OK;
@@ -748,9 +749,9 @@ static int launch_norm(const denet_opt_tensor_t* t, int64_t count, const Facts& 
     return DENET_OK;
 }
 
-// workspace: NORM_PARTS partial sums, one more for each launch (their shares are rounded up), the coefficient; then the clock of
+// workspace: NORM_NT_PARTS_BF16 partial sums, one more for each launch (their shares are rounded up), the coefficient; then the clock of
 // device-side counters
-static int64_t part_bytes(int64_t count) { return (NORM_PARTS + count / PACK + 1) * (int64_t)sizeof(double); }
+static int64_t part_bytes(int64_t count) { return (NORM_NT_PARTS_BF16 + count / PACK + 1) * (int64_t)sizeof(double); }
 static float* coef_in(void* ws, int64_t count) { return (float*)((char*)ws + part_bytes(count)); }
 static float* clock_in(void* ws, int64_t count) { return coef_in(ws, count) + 2; }
 
