@@ -88,7 +88,7 @@ class AdamWHyper(ctypes.Structure):
     """denet_adamw_t (include/denet_hip.h)."""
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
                 ("weight_decay", ctypes.c_double), ("max_norm", ctypes.c_double), ("device_steps", ctypes.c_int32),
-                ("reserved", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("step", ctypes.c_int64),
                 ("lr_dev", ctypes.c_void_p), ("coef", ctypes.c_void_p)]
 
 

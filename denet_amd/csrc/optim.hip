@@ -830,10 +830,10 @@ extern "C" int denet_grad_clip(const denet_opt_tensor_t* tensors, int64_t count,
     return over_packs(tensors, count, a, no_bias, [&](int chunks) { return launch(a, chunks); });
 }
 
-static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool host_steps) {
+static bool bad_tensor(const denet_opt_tensor_t& t, int bits, bool own_steps, bool device_steps) {
     if (bad_grad(t) || (t.param_dtype != DENET_F32 && t.param_dtype != DENET_BF16)) return true;
     if (t.n == 0) return false;
-    if (host_steps ? t.step < 1 : !t.step_dev || ((uintptr_t)t.step_dev & 7)) return true;
+    if ((own_steps && t.step < 1) || (device_steps && (!t.step_dev || ((uintptr_t)t.step_dev & 7)))) return true;
     if (!t.param || !t.exp_avg || !t.exp_avg_sq || ((uintptr_t)t.param & (t.param_dtype == DENET_F32 ? 3 : 1))) return true;
     if (((uintptr_t)t.exp_avg & 3) || ((uintptr_t)t.exp_avg_sq & 3)) return true;
     return bits == 8 && (!t.avg_scale || !t.sq_scale || ((uintptr_t)t.avg_scale & 3) || ((uintptr_t)t.sq_scale & 3));
@@ -852,17 +852,16 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
                                 float* norm, void* ws, int64_t ws_bytes, void* stream) {
     if (!h || bad_table(table) || (bits != 32 && bits != 8)) return DENET_E_BADARG;
     if (!(h->lr >= 0.) || !(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.) ||
-        !(h->weight_decay >= 0.) || h->max_norm != h->max_norm) return DENET_E_BADARG;
+        !(h->weight_decay >= 0.) || h->max_norm != h->max_norm || h->step < 0 || (h->step && h->device_steps)) return DENET_E_BADARG;
     Facts f;
     int rc = check_list(tensors, count, &f);
     if (rc != DENET_OK) return rc;
-    bool one_step = true;
-    int64_t t_one = 0;
+    // t of the whole list, 0 where it differs from tensor to tensor
+    const bool own_steps = !h->device_steps && !h->step;
+    int64_t t_all = h->step;
     for (int64_t i = 0; i < count; ++i) {
-        if (bad_tensor(tensors[i], bits, !h->device_steps)) return DENET_E_BADARG;
-        if (tensors[i].n == 0) continue;
-        if (!t_one) t_one = tensors[i].step;
-        one_step = one_step && tensors[i].step == t_one;
+        if (bad_tensor(tensors[i], bits, own_steps, h->device_steps)) return DENET_E_BADARG;
+        if (own_steps && tensors[i].n) t_all = !t_all || tensors[i].step == t_all ? tensors[i].step : -1;
     }
     const int64_t bytes = 2 * f.param_bytes + f.grad_bytes + f.elements * (bits == 8 ? 4 : 16);
     const bool clip = h->max_norm >= 0., nt = bytes >= NT_FROM, wide = bytes >= 12 * f.elements;
@@ -894,11 +893,11 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     }
     int64_t t_last = 0;
     float bias_last[2] = {0.f, 0.f};
-    auto bias = [&](const denet_opt_tensor_t& t, float out[2]) {
-        if (!h->device_steps && t.step != t_last) {
-            t_last = t.step;
-            bias_last[0] = (float)(h->lr / (1. - pow(h->beta1, (double)t.step)));
-            bias_last[1] = (float)(1. / sqrt(1. - pow(h->beta2, (double)t.step)));
+    auto bias_of = [&](int64_t t, float out[2]) {
+        if (t != t_last) {
+            t_last = t;
+            bias_last[0] = (float)(h->lr / (1. - pow(h->beta1, (double)t)));
+            bias_last[1] = (float)(1. / sqrt(1. - pow(h->beta2, (double)t)));
         }
         out[0] = bias_last[0];
         out[1] = bias_last[1];
@@ -914,15 +913,13 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
         a.eps = (float)h->eps;
         a.step_size = a.inv_bc2 = 0.f;
     };
-    if (table && (one_step || h->device_steps)) {
+    if (table && t_all >= 0) {
         AdamArgs<Tabled> a;
         fill(a);
         a.list = tabled(table, f.live);
         if (!h->device_steps) {
-            denet_opt_tensor_t t = {};
-            t.step = t_one;
             float b[2];
-            bias(t, b);
+            bias_of(t_all, b);
             a.step_size = b[0];
             a.inv_bc2 = b[1];
         }
@@ -932,6 +929,10 @@ extern "C" int denet_adamw_step(const denet_opt_tensor_t* tensors, int64_t count
     }
     AdamArgs<Packed> a;
     fill(a);
+    auto bias = [&](const denet_opt_tensor_t& t, float out[2]) {
+        if (h->device_steps) out[0] = out[1] = 0.f;
+        else bias_of(h->step ? h->step : t.step, out);
+    };
     return over_packs(tensors, count, a, bias, [&](int n) {
         launch_adamw(bits, nt, wide, n, a, st);
         DENET_CHECK_LAUNCH();

@@ -22,7 +22,7 @@ from ._lib import DenetHipError
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _W = _lib.OPT_TENSOR_WORDS
-_STEP, _STEP_DEV = 7, 8                                  # word indices in denet_opt_tensor_t
+_STEP = 7                                                # word index in denet_opt_tensor_t
 E4M3 = torch.float8_e4m3fn
 
 
@@ -138,12 +138,11 @@ class _List:
         self._run(name, self.table_addr, *args)
 
     def _run(self, name, *args):
-        fn = getattr(_lib.load(), name)
         if self.index != torch._C._cuda_getDevice():
             with torch.cuda.device(self.index):
-                rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
+                rc = getattr(_lib.load(), name)(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
         else:
-            rc = fn(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
+            rc = getattr(_lib.load(), name)(self.addr, self.count, *args, _lib.current_stream_handle(self.index))
         if rc != 0:
             raise DenetHipError(f"{name} failed: {_lib.strerror(rc)} (code {rc})")
 
@@ -174,7 +173,7 @@ class _Table(_List):
     def call(self, name, *args):
         if self.table is not None and _lib.current_stream_handle(self.index) != self.stream:
             self.table.record_stream(torch.cuda.current_stream(self.index))       # the plan may go while that stream still reads it
-        super().call(name, *args)
+        self._run(name, self.table_addr, *args)
 
 
 def _norm_limit(max_norm):
@@ -244,32 +243,41 @@ class _Update:
         self.h = _lib.AdamWHyper()
         self.h.device_steps = 1 if device_steps else 0
         self.addr = ctypes.addressof(self.h)
+        self.written = None                              # the numbers that `h` holds
 
-    def __call__(self, t, lr, betas, eps, weight_decay, max_norm, coef):
+    def __call__(self, t, step, lr, betas, eps, weight_decay, max_norm, coef):
+        """step: of every tensor; 0: the rows' own (or the device's counters)."""
         h = self.h
-        h.lr_dev = h.coef = None
         if isinstance(lr, torch.Tensor):
             if not self.device_steps:
                 raise DenetHipError("AdamW: lr as a tensor needs device step counters")
             h.lr_dev = _device_scalar(lr, "lr", t.device)
-            self.lr = lr
-        else:
-            h.lr = lr
-        h.beta1, h.beta2 = betas
-        h.eps, h.weight_decay = eps, weight_decay
+            self.lr, lr = lr, 0.0
+        elif self.device_steps:
+            h.lr_dev = None
         if coef is not None:
             if max_norm is not None:
                 raise DenetHipError("AdamW: max_norm or coef, not both")
             h.coef = _device_scalar(coef, "coef", t.device)
-        norm, ws = None, None
-        h.max_norm = -1.0
-        if max_norm is not None:
-            h.max_norm = _norm_limit(max_norm)
-            norm = t.scalar()
-        if norm is not None or self.device_steps:
-            ws = t.ws()
-        t.call("denet_adamw_step", self.bits, self.addr, norm.data_ptr() if norm is not None else None,
-               ws.data_ptr() if ws is not None else None, t.ws_bytes if ws is not None else 0)
+        limit = -1.0 if max_norm is None else _norm_limit(max_norm)
+        numbers = (step, lr, *betas, eps, weight_decay, limit)
+        if numbers != self.written:
+            self.written = None
+            h.step, h.lr, h.beta1, h.beta2, h.eps, h.weight_decay, h.max_norm = numbers
+            self.written = numbers
+        norm = ws = None
+        try:
+            if max_norm is not None:
+                norm, ws = t.scalar(), t.ws()
+                t.call("denet_adamw_step", self.bits, self.addr, norm.data_ptr(), ws.data_ptr(), t.ws_bytes)
+            elif self.device_steps:
+                ws = t.ws()
+                t.call("denet_adamw_step", self.bits, self.addr, None, ws.data_ptr(), t.ws_bytes)
+            else:
+                t.call("denet_adamw_step", self.bits, self.addr, None, None, 0)
+        finally:
+            if coef is not None:
+                h.coef = None
         return norm
 
 
@@ -328,7 +336,6 @@ class AdamWPlan:
         self._versioned = [t for t in params if not t.is_inference()]
         self._table = (_List if _once else _Table)(rows, n, device, index, lists)
         self._update = _Update(self.bits, steps is not None)
-        self._step = 1
 
     def step(self, step=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, coef=None):
         """One update.  step: the number t >= 1 of this update (an int, or one per parameter); not with device counters.  lr: a number, or (with
@@ -343,27 +350,24 @@ class AdamWPlan:
             if torch.cuda.is_current_stream_capturing():
                 raise DenetHipError("AdamWPlan.step: a captured step would repeat its step number at every replay; give the plan "
                                     "device step counters (`steps`)")
-            self._set_steps(step)
-        norm = self._update(self._table, lr, betas, eps, weight_decay, max_norm, coef)
+            step = self._one_step(step)
+        norm = self._update(self._table, step or 0, lr, betas, eps, weight_decay, max_norm, coef)
         if self._versioned:
             torch.autograd.graph.increment_version(self._versioned)
         return norm
 
-    def _set_steps(self, step):
-        t = self._table
+    def _one_step(self, step):
+        """The step number of every parameter; 0 where they differ (the rows then hold them)."""
         if not isinstance(step, (list, tuple)):
             step = int(step)
-            if step != self._step:
-                if step < 1:
-                    raise DenetHipError(f"AdamWPlan.step: the first step is 1, got {step}")
-                t.buf[_STEP::_W] = array.array("q", [step]) * t.count
-                self._step = step
-            return
-        step = [int(s) for s in step]
+            if step < 1:
+                raise DenetHipError(f"AdamWPlan.step: the first step is 1, got {step}")
+            return step
+        step, t = [int(x) for x in step], self._table
         if len(step) != t.count or min(step) < 1:
             raise DenetHipError(f"AdamWPlan.step: {t.count} step numbers >= 1 are needed")
         t.buf[_STEP::_W] = array.array("q", step)
-        self._step = None
+        return 0
 
 
 def grad_norm(grads):

@@ -125,10 +125,10 @@ class AdamW(torch.optim.Optimizer):
         max_norm, coef, self.grad_norm = self.max_norm, None, None
         if max_norm is not None and len(lists) > 1:
             # one norm over all groups: its coefficient stays on the device for the groups' calls
-            self.grad_norm, coef = GradNormPlan([g for _, _, _, grads, _ in lists for g in grads], _once=True).norm_and_coef(max_norm)
+            self.grad_norm, coef = GradNormPlan([g for _, _, _, grads, _, _ in lists for g in grads], _once=True).norm_and_coef(max_norm)
             max_norm = None
-        for group, table, params, _, states in lists:
-            norm = self._update(table, group["lr"], group["betas"], group["eps"], group["weight_decay"], max_norm, coef)
+        for group, table, params, _, states, one in lists:
+            norm = self._update(table, one, group["lr"], group["betas"], group["eps"], group["weight_decay"], max_norm, coef)
             if max_norm is not None:
                 self.grad_norm = norm
             if not self.capturable:
@@ -138,12 +138,12 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _list_of(self, group, capturing):
-        """(table, parameters, gradients, states) of the group's parameters that have a gradient; None if none has.  Everything the
-        kernels rely on is checked at every step."""
+        """(table, parameters, gradients, states, number of the step or 0 where it differs) of the group's parameters that have a
+        gradient; None if none has.  Everything the kernels rely on is checked at every step."""
         state, eight, counted = self.state, self.state_bits == 8, self.capturable
         k_avg, k_sq = "exp_avg", "exp_avg_sqrt" if eight else "exp_avg_sq"
         types = {E4M3} if eight else {torch.float32}
-        params, grads, states, rows, index = [], [], [], [], None
+        params, grads, states, rows, index, one = [], [], [], [], None, None
         for p in group["params"]:
             g = p.grad
             if g is None:
@@ -182,13 +182,15 @@ class AdamW(torch.optim.Optimizer):
                 step_dev, step = step.data_ptr(), 1
             else:
                 step = s["step"] + 1
+                if step != one:
+                    one = step if one is None else 0
             states.append(s)
             params.append(p)
             grads.append(g)
             rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n, step, step_dev, _CODE[p.dtype] | (_CODE[g.dtype] << 32))
         if not params:
             return None
-        return _List(rows, len(params), device, index), params, grads, states
+        return _List(rows, len(params), device, index), params, grads, states, one or 0
 
     # ---- checkpoints --------------------------------------------------------------------------------
     def load_state_dict(self, state_dict):

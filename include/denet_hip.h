@@ -403,7 +403,7 @@ typedef struct denet_opt_tensor {
     float* avg_scale;
     float* sq_scale;
     int64_t n;              /* elements, < 2^48                                                   */
-    int64_t step;           /* t >= 1 of this update                                              */
+    int64_t step;           /* t >= 1 of this update, where denet_adamw_t.step is 0               */
     int64_t* step_dev;      /* with denet_adamw_t.device_steps: device counter of the updates done so far, advanced by
                                the call, in place of `step` -- for calls that a captured graph replays */
     int32_t param_dtype;
@@ -415,6 +415,7 @@ typedef struct denet_adamw {
                                are not written)                                                   */
     int32_t device_steps;   /* 1: the tensors' step_dev count                                      */
     int32_t reserved;
+    int64_t step;           /* t >= 1 of this update for every tensor; 0: each has its own         */
     const float* lr_dev;    /* with device_steps: device scalar read instead of lr, or NULL        */
     const float* coef;      /* device scalar: coefficient that denet_grad_norm left, where one norm spans several
                                calls (parameter groups); or NULL.  Not together with max_norm >= 0 */

@@ -86,6 +86,7 @@ def test_abi_refuses_bad_steps(bits):
     assert call(max_norm=1.0, norm=NORM) == BADARG                                          # no workspace
     assert call(max_norm=1.0, norm=NORM, ws=WS, ws_bytes=need - 1) == WORKSPACE
     assert call(max_norm=1.0, norm=NORM, ws=WS, ws_bytes=need, coef=NORM) == BADARG         # both kinds of clipping
+    assert call(step=-1) == BADARG and call(step=1, device_steps=1, ws=WS, ws_bytes=need) == BADARG
     assert call(lr_dev=NORM) == BADARG                                                      # lr on the device without counters there
     assert call(device_steps=1, ws=WS, ws_bytes=need) == BADARG                             # no counter
     assert call(dict(step_dev=0x90004), device_steps=1, ws=WS, ws_bytes=need) == BADARG
