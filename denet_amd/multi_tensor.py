@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import operator
 from bisect import bisect_right
 
 import torch
@@ -359,11 +360,11 @@ class AdamWPlan:
     def _one_step(self, step):
         """The step number of every parameter; 0 where they differ (the rows then hold them)."""
         if not isinstance(step, (list, tuple)):
-            step = int(step)
+            step = operator.index(step)
             if step < 1:
                 raise DenetHipError(f"AdamWPlan.step: the first step is 1, got {step}")
             return step
-        step, t = [int(x) for x in step], self._table
+        step, t = [operator.index(x) for x in step], self._table
         if len(step) != t.count or min(step) < 1:
             raise DenetHipError(f"AdamWPlan.step: {t.count} step numbers >= 1 are needed")
         t.buf[_STEP::_W] = array.array("q", step)

@@ -610,6 +610,52 @@ def test_streams_beyond_the_cache(bits, pt, gt, dev):
     assert all(torch.equal(a, b) for a, b in zip(d["g"], ref))
 
 
+def test_norms_of_one_plan_on_two_streams_at_once(dev):
+    from denet_amd import ops
+    grads, _, _ = _grads([7, 300_001, 2_000_003] * 20, [F32, BF16], dev, 37, 1)
+    plan = ops.GradNormPlan(grads)
+    want = plan.norm()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(30):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(plan.norm())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+def test_plans_from_two_threads(dev):
+    """Host calls from two threads at once, each on a stream and a plan of its own."""
+    import threading
+    sets = [_inputs([4097, 5, 70_001], F32, F32, 8, dev, 38 + k) for k in range(2)]
+    refs = [_clone(d) for d in sets]
+    torch.cuda.synchronize()
+    fails = []
+
+    def work(d):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                plan = _plan(d, 8)
+                for t in range(1, 60):
+                    plan.step(t, max_norm=0.01, **H)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                           # (an exception in a thread would pass unseen)
+            fails.append(e)
+
+    threads = [threading.Thread(target=work, args=(d,)) for d in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not fails
+    for d, r in zip(sets, refs):
+        plan = _plan(r, 8)
+        for t in range(1, 60):
+            plan.step(t, max_norm=0.01, **H)
+        assert all(_same(a, b) for k in r for a, b in zip(d[k], r[k]))
+
+
 def test_a_plan_may_go_while_another_stream_uses_it(dev):
     from denet_amd import ops
     g = torch.ones(200_000_000, device=dev)
