@@ -335,7 +335,9 @@ class AdamWPlan:
         codes = [_CODE[p.dtype] | (_CODE[g.dtype] << 32) for p, g in zip(params, grads)]
         rows = [w for row in zip(at[0], at[1], at[2], at[3], scales[0], scales[1], sizes, [1] * n, counters, codes) for w in row]
         self._versioned = [t for t in params if not t.is_inference()]
-        self._table = (_List if _once else _Table)(rows, n, device, index, lists)
+        # (the parameters' storages too: `module.to(...)` replaces them under the same objects, and the plan would write to freed memory)
+        keep = lists if _once else lists + [[p.untyped_storage() for p in params]]
+        self._table = (_List if _once else _Table)(rows, n, device, index, keep)
         self._update = _Update(self.bits, steps is not None)
 
     def step(self, step=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, coef=None):

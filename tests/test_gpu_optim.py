@@ -965,3 +965,16 @@ def test_trainer_clips_for_any_optimizer(dev, tmp_path):
     plain = _trainer(tmp_path, dict(name="sgd", lr=0.1))
     plain.step(plain.train_loader.batch(0), train=True)
     assert plain.grad_norm is None
+
+
+def test_a_plan_keeps_the_memory_that_it_writes(dev):
+    """A parameter whose data is replaced under a plan: the plan still writes to the old memory, which must not have become another
+    tensor's."""
+    d = _inputs([5_000_000], F32, F32, 32, dev, 60)
+    plan = _plan(d, 32)
+    old = d["p"][0].data_ptr()
+    d["p"][0].data = torch.zeros(5_000_000, device=dev)
+    other = [torch.zeros(5_000_000, device=dev) for _ in range(3)]
+    assert all(x.data_ptr() != old for x in other) and d["p"][0].data_ptr() != old
+    plan.step(1, **H)
+    assert all(float(x.abs().sum()) == 0 for x in other) and float(d["p"][0].abs().sum()) == 0
