@@ -6,8 +6,8 @@ name=$1; shift
 root=$(cd "$(dirname "$0")/../.." && pwd)
 out=$root/build/alt_$name
 mkdir -p $out
-for f in api masked_sum proto_extend classify upsample_loss metrics head_step; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -fPIC -Wall -Wno-unused-function "$@" \
+for f in api masked_sum proto_extend classify upsample_loss metrics head_step optim; do
+  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Wall -Wno-unused-function "$@" \
       -c $root/denet_amd/csrc/$f.hip -o $out/$f.o &
 done
 wait
